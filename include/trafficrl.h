@@ -858,6 +858,114 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
                      double* ep_reward, double* ep_tstt_sum, double* ep_auc, double* ep_prev_tstt, int64_t* ep_len,
                      uint8_t* finished, void* stream);
 
+/* ------------------------------------------------ attention between nodes
+ * Softmax attention of query rows over the nodes of their own network, for a
+ * packed batch of networks of any sizes (the global counterpart of the edge
+ * attention in trx_gat_forward).  Graph b's query rows are q_ptr[b] ..
+ * q_ptr[b+1] and its key rows k_ptr[b] .. k_ptr[b+1] (int64, non-decreasing,
+ * device; values outside the tensors are clamped).  For query row i (in its
+ * graph), key row j, head h (key/value head h / (heads / kv_heads)):
+ *   z = scale <q_i, k_j>;  z = cap tanh(z / cap) if cap > 0
+ *   w = z - slope[h] d_ij;  out_i = sum_j softmax_j(w) v_j
+ * d_ij = dist[b * dist_graph + i * dist_row + j] (elements; dist_graph 0: one
+ * matrix for every graph); pair (i, j) is seen where i < dist_rows, j <
+ * dist_cols and d_ij is finite (dist NULL: every pair, no bias; slope NULL:
+ * no bias).  A row that sees nothing, or only scores of -inf, gives zeros and
+ * passes no gradient; so do the rows of no graph.
+ * q, k, v: dtype (0 float32, 1 bfloat16, 2 float16), row and head strides in
+ * elements (multiples of 16 bytes, like the pointers), channels contiguous,
+ * channels a multiple of 8 up to TRX_ATT_MAX_CHANNELS.  out, grad_out,
+ * grad_q [num_queries, heads, channels], grad_k, grad_v [num_nodes, kv_heads,
+ * channels]: contiguous, in dtype.  lse float32 [num_queries, heads]:
+ * log2(sum_j 2^(w log2 e)), written by the forward where not NULL (-inf for an
+ * empty row), read by the backward.  grad_slope float32 [heads] or NULL.
+ * max_queries / max_nodes: the largest graph's rows; they only shape the
+ * launch (a smaller value costs time, never rows).  Sums and the softmax's
+ * statistics are float32; probabilities and score gradients enter the matrix
+ * products in dtype.  Deterministic: no float atomics.  workspace:
+ * trx_node_attention_workspace_bytes(args, backward) bytes, 16-byte aligned
+ * (0: may be NULL).                                                        */
+#define TRX_ATT_MAX_CHANNELS 128
+typedef struct trx_node_attention_args {
+    int32_t num_graphs, heads, kv_heads, channels, dtype;
+    int32_t dist_rows, dist_cols;
+    float scale, cap;
+    int64_t max_queries, max_nodes, num_queries, num_nodes;
+    const void *q, *k, *v;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    const int64_t *q_ptr, *k_ptr;       /* [num_graphs + 1] */
+    const float* dist;
+    int64_t dist_graph, dist_row;
+    const float* slope;                 /* [heads] */
+    void* out;
+    float* lse;
+    const void* grad_out;
+    void *grad_q, *grad_k, *grad_v;
+    float* grad_slope;
+    void* workspace;
+    int64_t workspace_bytes;
+} trx_node_attention_args;
+int64_t trx_node_attention_workspace_bytes(const trx_node_attention_args* a, int32_t backward);
+int trx_node_attention_forward(const trx_node_attention_args* a, void* stream);
+int trx_node_attention_backward(const trx_node_attention_args* a, void* stream);
+
+/* ------------------------------------------- log probabilities of actions
+ * The masked categorical policy over each row's links (the softmax of
+ * src/rl/sac.py:44-46 with its log, entropy and ranking).  logits: dtype (0
+ * float32, 1 bfloat16, 2 float16); row r is logits + r * row_stride of
+ * row_len elements (row_ptr NULL), or elements row_ptr[r] .. row_ptr[r+1] of
+ * a packed vector of `total` (int64, non-decreasing, device; clamped).  A link
+ * may be chosen where its mask is > 0 (mask_dtype 0: float32, 1: uint8; laid
+ * out like the logits with mask_stride; NULL: every link) and its logit is
+ * not -inf.  Over those, with p = softmax:
+ *   log_prob[r] = log p[action[r]] (-inf where that link may not be chosen or
+ *     is outside the row), entropy[r] = -sum p log p (0 for an empty row),
+ *   top_log_prob / top_action [rows, top_k]: the highest log probabilities in
+ *     falling order and their links (row-local; ties: the lower link first; -inf
+ *     and -1 where fewer links may be chosen), top_k 0..TRX_TOP_MAX.
+ * stats float32 [rows, 4]: saved for the backward.  float32 throughout.
+ * Backward: grad_logits (dtype; rows contiguous, row_len apart, or packed like
+ * the logits) = g_log_prob (1[j = action] - p_j) - g_entropy p_j (log p_j +
+ * entropy) + sum_t g_top[t] (1[j = top_action[t]] - p_j); 0 where a link may
+ * not be chosen, and for packed elements of no row; an action of log_prob -inf
+ * passes nothing.  The g_* may be NULL.  max_row: the longest packed row; it
+ * only shapes the launch.  workspace: trx_action_log_probs_workspace_bytes
+ * bytes, 16-byte aligned (0: may be NULL; the forward's only).             */
+#define TRX_TOP_MAX 16
+typedef struct trx_action_log_probs_args {
+    int64_t rows, row_len, row_stride, total, max_row, mask_stride;
+    int32_t dtype, mask_dtype, top_k, _pad;
+    const void* logits;
+    const void* mask;
+    const int64_t* row_ptr;
+    const int64_t* action;
+    float *log_prob, *entropy, *stats, *top_log_prob;
+    int64_t* top_action;
+    const float *g_log_prob, *g_entropy, *g_top;
+    void* grad_logits;
+    void* workspace;
+    int64_t workspace_bytes;
+} trx_action_log_probs_args;
+int64_t trx_action_log_probs_workspace_bytes(const trx_action_log_probs_args* a);
+int trx_action_log_probs_forward(const trx_action_log_probs_args* a, void* stream);
+int trx_action_log_probs_backward(const trx_action_log_probs_args* a, void* stream);
+
+/* ------------------------------------------------------ dropout + residual
+ * y = residual + keep * x * 65536 / (65536 - border) over n elements (dtype 0
+ * float32, 1 bfloat16, 2 float16; residual may be NULL), computed in float32
+ * and rounded once.  Element e is kept where its 16 random bits are >= border
+ * (0..65535: a drop probability of border / 65536): half e % 8 (low half
+ * first) of the four words of Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011)
+ * with counter (e / 8 low, e / 8 high, step mod 2^32, site) and key (seed low,
+ * seed high).  rng int64 [2] (device): (seed, step); the forward writes the
+ * pair it used to rng_used, from which the backward, grad_x = keep * grad_y *
+ * 65536 / (65536 - border), draws the same bits again: no mask is stored and
+ * rng may move on in between.  Pointers aligned to 16 bytes.               */
+int trx_dropout_add_forward(int64_t n, int32_t dtype, const void* x, const void* residual, const int64_t* rng,
+                            int32_t border, uint32_t site, void* y, int64_t* rng_used, void* stream);
+int trx_dropout_add_backward(int64_t n, int32_t dtype, const void* grad_y, const int64_t* rng_used, int32_t border,
+                             uint32_t site, void* grad_x, void* stream);
+
 /* ------------------------------------------------------ graph support
  * Rewrites every memset node of a captured, not yet instantiated hipGraph_t
  * (passed as void*) into an equivalent fill-kernel node with the same

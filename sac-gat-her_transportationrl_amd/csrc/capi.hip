@@ -1321,6 +1321,170 @@ int trx_sac_adam(const trx_adam_args* a, void* stream) {
     return TRX_OK;
 }
 
+namespace {
+
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
+// shapes that the workspace size depends on
+int check_attention_shape(const trx_node_attention_args* a) {
+    if (!a) return fail(TRX_EINVAL, "node_attention: args is NULL");
+    if (a->num_graphs < 0 || a->num_queries < 0 || a->num_nodes < 0 || a->max_queries < 0 || a->max_nodes < 0)
+        return fail(TRX_EINVAL, "node_attention: negative size");
+    if (a->dtype < 0 || a->dtype > 2) return fail(TRX_EINVAL, "node_attention: dtype %d", a->dtype);
+    if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0)
+        return fail(TRX_EINVAL, "node_attention: kv_heads (%d) must divide heads (%d)", a->kv_heads, a->heads);
+    if (a->heads > 1024) return fail(TRX_EUNSUP, "node_attention: at most 1024 heads (got %d)", a->heads);
+    if (a->channels < 8 || a->channels > TRX_ATT_MAX_CHANNELS || a->channels % 8 != 0)
+        return fail(TRX_EUNSUP, "node_attention: channels must be a multiple of 8 up to %d (got %d)",
+                    TRX_ATT_MAX_CHANNELS, a->channels);
+    if (a->num_queries > (int64_t(1) << 31) - 1 || a->num_nodes > (int64_t(1) << 31) - 1)
+        return fail(TRX_EUNSUP, "node_attention: at most 2^31 - 1 rows");
+    if (a->num_graphs > (1 << 24)) return fail(TRX_EUNSUP, "node_attention: at most 2^24 graphs");
+    return TRX_OK;
+}
+
+int check_attention(const trx_node_attention_args* a, bool backward) {
+    int rc = check_attention_shape(a);
+    if (rc) return rc;
+    if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0.0f)
+        return fail(TRX_EINVAL, "node_attention: scale must be finite and cap finite and >= 0");
+    if (!a->q_ptr || !a->k_ptr) return fail(TRX_EINVAL, "node_attention: NULL q_ptr / k_ptr");
+    if (a->num_queries > 0 && (!a->q || !a->out)) return fail(TRX_EINVAL, "node_attention: NULL q / out");
+    if (a->num_nodes > 0 && (!a->k || !a->v)) return fail(TRX_EINVAL, "node_attention: NULL k / v");
+    const int64_t unit = a->dtype == 0 ? 4 : 8;   // elements per 16 bytes
+    for (int64_t s : {a->q_row, a->q_head, a->k_row, a->k_head, a->v_row, a->v_head})
+        if (s < 0 || s % unit != 0)
+            return fail(TRX_EINVAL, "node_attention: strides must be multiples of 16 bytes and not negative");
+    for (const void* p : {a->q, a->k, a->v, (const void*)a->out, a->grad_out, (const void*)a->grad_q,
+                          (const void*)a->grad_k, (const void*)a->grad_v, (const void*)a->workspace})
+        if (misaligned(p)) return fail(TRX_EINVAL, "node_attention: buffers must be 16-byte aligned");
+    if (a->dist && (a->dist_rows < 0 || a->dist_cols < 0 || a->dist_row < 0 || a->dist_graph < 0))
+        return fail(TRX_EINVAL, "node_attention: negative dist shape or stride");
+    if (backward) {
+        if (a->num_queries > 0 && (!a->lse || !a->grad_out || !a->grad_q))
+            return fail(TRX_EINVAL, "node_attention: NULL lse / grad_out / grad_q");
+        if (a->num_nodes > 0 && (!a->grad_k || !a->grad_v)) return fail(TRX_EINVAL, "node_attention: NULL grad_k / grad_v");
+    }
+    const size_t need = trx::node_attention_workspace(*a, backward);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < (int64_t)need))
+        return fail(TRX_EINVAL, "node_attention: workspace of %lld bytes, %zu needed",
+                    a->workspace ? (long long)a->workspace_bytes : 0LL, need);
+    return TRX_OK;
+}
+
+int check_log_probs_shape(const trx_action_log_probs_args* a) {
+    if (!a) return fail(TRX_EINVAL, "action_log_probs: args is NULL");
+    if (a->rows < 0 || a->row_len < 0 || a->row_stride < 0 || a->total < 0 || a->max_row < 0 || a->mask_stride < 0)
+        return fail(TRX_EINVAL, "action_log_probs: negative size");
+    if (a->rows > (int64_t(1) << 31) - 1) return fail(TRX_EUNSUP, "action_log_probs: at most 2^31 - 1 rows");
+    if (a->row_len > (int64_t(1) << 30) || a->max_row > (int64_t(1) << 30))
+        return fail(TRX_EUNSUP, "action_log_probs: at most 2^30 links in a row");
+    if (a->dtype < 0 || a->dtype > 2 || a->mask_dtype < 0 || a->mask_dtype > 1)
+        return fail(TRX_EINVAL, "action_log_probs: dtype %d, mask_dtype %d", a->dtype, a->mask_dtype);
+    if (a->top_k < 0 || a->top_k > TRX_TOP_MAX)
+        return fail(TRX_EUNSUP, "action_log_probs: top_k must be 0..%d (got %d)", TRX_TOP_MAX, a->top_k);
+    return TRX_OK;
+}
+
+int check_log_probs(const trx_action_log_probs_args* a, bool backward) {
+    int rc = check_log_probs_shape(a);
+    if (rc) return rc;
+    if (a->rows > 0) {
+        if (!a->logits && (a->row_ptr ? a->total : a->row_len) > 0) return fail(TRX_EINVAL, "action_log_probs: NULL logits");
+        if (!a->action || !a->stats || !a->log_prob || !a->entropy)
+            return fail(TRX_EINVAL, "action_log_probs: NULL action / log_prob / entropy / stats");
+        if (a->top_k > 0 && !a->top_action) return fail(TRX_EINVAL, "action_log_probs: NULL top_action");
+        if (!backward && a->top_k > 0 && !a->top_log_prob) return fail(TRX_EINVAL, "action_log_probs: NULL top_log_prob");
+    }
+    if (backward && !a->grad_logits && (a->row_ptr ? a->total : a->rows * a->row_len) > 0)
+        return fail(TRX_EINVAL, "action_log_probs: NULL grad_logits");
+    if (!backward) {
+        const size_t need = trx::action_log_probs_workspace(*a);
+        if (need > 0 && (!a->workspace || misaligned(a->workspace) || a->workspace_bytes < (int64_t)need))
+            return fail(TRX_EINVAL, "action_log_probs: workspace of %lld bytes, %zu needed",
+                        a->workspace ? (long long)a->workspace_bytes : 0LL, need);
+    }
+    return TRX_OK;
+}
+
+int check_dropout(int64_t n, int32_t dtype, const void* x, const int64_t* rng, int32_t border, const void* y) {
+    if (n < 0 || dtype < 0 || dtype > 2) return fail(TRX_EINVAL, "dropout_add: n >= 0, dtype 0..2");
+    if (n > (int64_t(1) << 40)) return fail(TRX_EUNSUP, "dropout_add: at most 2^40 elements");
+    if (border < 0 || border > 65535) return fail(TRX_EINVAL, "dropout_add: border must be 0..65535 (got %d)", border);
+    if (n > 0 && (!x || !rng || !y)) return fail(TRX_EINVAL, "dropout_add: NULL buffer");
+    if (misaligned(x) || misaligned(y)) return fail(TRX_EINVAL, "dropout_add: buffers must be 16-byte aligned");
+    return TRX_OK;
+}
+
+}  // namespace
+
+int64_t trx_node_attention_workspace_bytes(const trx_node_attention_args* a, int32_t backward) {
+    return check_attention_shape(a) ? -1 : (int64_t)trx::node_attention_workspace(*a, backward != 0);
+}
+
+int trx_node_attention_forward(const trx_node_attention_args* a, void* stream) {
+    int rc = check_attention(a, false);
+    if (rc) return rc;
+    if (a->num_queries == 0) return TRX_OK;
+    hipError_t e = trx::launch_node_attention_fwd(*a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(TRX_EHIP, "node_attention forward launch: %s", hipGetErrorString(e));
+    return TRX_OK;
+}
+
+int trx_node_attention_backward(const trx_node_attention_args* a, void* stream) {
+    int rc = check_attention(a, true);
+    if (rc) return rc;
+    hipError_t e = trx::launch_node_attention_bwd(*a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(TRX_EHIP, "node_attention backward launch: %s", hipGetErrorString(e));
+    return TRX_OK;
+}
+
+int64_t trx_action_log_probs_workspace_bytes(const trx_action_log_probs_args* a) {
+    return check_log_probs_shape(a) ? -1 : (int64_t)trx::action_log_probs_workspace(*a);
+}
+
+int trx_action_log_probs_forward(const trx_action_log_probs_args* a, void* stream) {
+    int rc = check_log_probs(a, false);
+    if (rc) return rc;
+    if (a->rows == 0) return TRX_OK;
+    hipError_t e = trx::launch_action_log_probs_fwd(*a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(TRX_EHIP, "action_log_probs forward launch: %s", hipGetErrorString(e));
+    return TRX_OK;
+}
+
+int trx_action_log_probs_backward(const trx_action_log_probs_args* a, void* stream) {
+    int rc = check_log_probs(a, true);
+    if (rc) return rc;
+    if ((a->row_ptr ? a->total : a->rows * a->row_len) == 0) return TRX_OK;
+    hipError_t e = trx::launch_action_log_probs_bwd(*a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(TRX_EHIP, "action_log_probs backward launch: %s", hipGetErrorString(e));
+    return TRX_OK;
+}
+
+int trx_dropout_add_forward(int64_t n, int32_t dtype, const void* x, const void* residual, const int64_t* rng,
+                            int32_t border, uint32_t site, void* y, int64_t* rng_used, void* stream) {
+    int rc = check_dropout(n, dtype, x, rng, border, y);
+    if (rc) return rc;
+    if (n > 0 && (!rng_used || misaligned(residual)))
+        return fail(TRX_EINVAL, "dropout_add: NULL rng_used or a residual that is not 16-byte aligned");
+    if (n == 0) return TRX_OK;
+    hipError_t e = trx::launch_dropout_add(n, dtype, x, residual, rng, border, site, y, rng_used,
+                                           static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(TRX_EHIP, "dropout_add forward launch: %s", hipGetErrorString(e));
+    return TRX_OK;
+}
+
+int trx_dropout_add_backward(int64_t n, int32_t dtype, const void* grad_y, const int64_t* rng_used, int32_t border,
+                             uint32_t site, void* grad_x, void* stream) {
+    int rc = check_dropout(n, dtype, grad_y, rng_used, border, grad_x);
+    if (rc) return rc;
+    if (n == 0) return TRX_OK;
+    hipError_t e = trx::launch_dropout_add(n, dtype, grad_y, nullptr, rng_used, border, site, grad_x, nullptr,
+                                           static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(TRX_EHIP, "dropout_add backward launch: %s", hipGetErrorString(e));
+    return TRX_OK;
+}
+
 int trx_graph_patch_memsets(void* hip_graph, int32_t* n_patched) {
     if (!hip_graph) return fail(TRX_EINVAL, "graph_patch_memsets: NULL graph");
     int n = 0;

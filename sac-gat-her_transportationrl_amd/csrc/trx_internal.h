@@ -263,4 +263,13 @@ hipError_t launch_per32_sample_weighted(const float* tree, int64_t capacity, con
                                         double beta, int64_t* out_idx, float* out_pri, float* out_w,
                                         hipStream_t stream);
 
+size_t node_attention_workspace(const trx_node_attention_args& a, bool backward);
+hipError_t launch_node_attention_fwd(const trx_node_attention_args& a, hipStream_t stream);
+hipError_t launch_node_attention_bwd(const trx_node_attention_args& a, hipStream_t stream);
+size_t action_log_probs_workspace(const trx_action_log_probs_args& a);
+hipError_t launch_action_log_probs_fwd(const trx_action_log_probs_args& a, hipStream_t stream);
+hipError_t launch_action_log_probs_bwd(const trx_action_log_probs_args& a, hipStream_t stream);
+hipError_t launch_dropout_add(int64_t n, int dtype, const void* x, const void* residual, const int64_t* rng, int border,
+                              uint32_t site, void* y, int64_t* rng_used, hipStream_t stream);
+
 }  // namespace trx

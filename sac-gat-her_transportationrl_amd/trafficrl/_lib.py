@@ -37,6 +37,9 @@ EXPORTS = (
     "trx_gat_layer0_infer", "trx_gat_layer0_prepare", "trx_gat_mid_infer",
     "trx_gat_layer_infer_multi", "trx_edge_head_infer_multi", "trx_edge_head_backward_multi",
     "trx_gat_prologue_infer_multi", "trx_gat_layer_backward_multi", "trx_gat_prologue_backward_multi",
+    "trx_node_attention_workspace_bytes", "trx_node_attention_forward", "trx_node_attention_backward",
+    "trx_action_log_probs_workspace_bytes", "trx_action_log_probs_forward", "trx_action_log_probs_backward",
+    "trx_dropout_add_forward", "trx_dropout_add_backward",
 )
 MAX_NETS = 6   # TRX_MAX_NETS: networks per *_multi launch (ABI 11)
 
@@ -245,6 +248,37 @@ class TrxPsumList(ctypes.Structure):
     ]
 
 
+ATT_MAX_CHANNELS = 128   # TRX_ATT_MAX_CHANNELS
+TOP_MAX = 16             # TRX_TOP_MAX
+_i64 = ctypes.c_int64
+
+
+class TrxNodeAttentionArgs(ctypes.Structure):
+    """trx_node_attention_args (include/trafficrl.h)."""
+    _fields_ = [
+        ("num_graphs", _i32), ("heads", _i32), ("kv_heads", _i32), ("channels", _i32), ("dtype", _i32),
+        ("dist_rows", _i32), ("dist_cols", _i32), ("scale", _f32), ("cap", _f32),
+        ("max_queries", _i64), ("max_nodes", _i64), ("num_queries", _i64), ("num_nodes", _i64),
+        ("q", _vp), ("k", _vp), ("v", _vp), ("q_row", _i64), ("q_head", _i64), ("k_row", _i64), ("k_head", _i64),
+        ("v_row", _i64), ("v_head", _i64), ("q_ptr", _vp), ("k_ptr", _vp),
+        ("dist", _vp), ("dist_graph", _i64), ("dist_row", _i64), ("slope", _vp), ("out", _vp), ("lse", _vp),
+        ("grad_out", _vp), ("grad_q", _vp), ("grad_k", _vp), ("grad_v", _vp), ("grad_slope", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class TrxActionLogProbsArgs(ctypes.Structure):
+    """trx_action_log_probs_args (include/trafficrl.h)."""
+    _fields_ = [
+        ("rows", _i64), ("row_len", _i64), ("row_stride", _i64), ("total", _i64), ("max_row", _i64),
+        ("mask_stride", _i64), ("dtype", _i32), ("mask_dtype", _i32), ("top_k", _i32), ("_pad", _i32),
+        ("logits", _vp), ("mask", _vp), ("row_ptr", _vp), ("action", _vp),
+        ("log_prob", _vp), ("entropy", _vp), ("stats", _vp), ("top_log_prob", _vp), ("top_action", _vp),
+        ("g_log_prob", _vp), ("g_entropy", _vp), ("g_top", _vp), ("grad_logits", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 MAX_COPY = 16
 
 
@@ -374,6 +408,14 @@ def load():
     L.trx_layer_tail_workspace_floats.restype = ctypes.c_int64
     L.trx_layer_tail_backward.argtypes = [_i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                           _vp]
+    for name, st in (("trx_node_attention_", TrxNodeAttentionArgs), ("trx_action_log_probs_", TrxActionLogProbsArgs)):
+        getattr(L, name + "workspace_bytes").restype = ctypes.c_int64
+        getattr(L, name + "workspace_bytes").argtypes = [ctypes.POINTER(st)]
+        for step in ("forward", "backward"):
+            getattr(L, name + step).argtypes = [ctypes.POINTER(st), _vp]
+    L.trx_node_attention_workspace_bytes.argtypes = [ctypes.POINTER(TrxNodeAttentionArgs), _i32]
+    L.trx_dropout_add_forward.argtypes = [_i64, _i32, _vp, _vp, _vp, _i32, ctypes.c_uint32, _vp, _vp, _vp]
+    L.trx_dropout_add_backward.argtypes = [_i64, _i32, _vp, _vp, _i32, ctypes.c_uint32, _vp, _vp]
     for name in ("trx_graph_create", "trx_graph_destroy", "trx_graph_info", "trx_assign", "trx_reset", "trx_step",
                  "trx_observe", "trx_gat_forward", "trx_gat_backward", "trx_per_update", "trx_per_sample",
                  "trx_graph_patch_memsets", "trx_gat_layer_infer", "trx_edge_head_infer", "trx_gat_prologue_infer",
@@ -385,7 +427,9 @@ def load():
                  "trx_per32_sample", "trx_per32_sample_weighted", "trx_damage_sample", "trx_multi_gather",
                  "trx_episode_step", "trx_gat_layer_backward", "trx_partial_sum", "trx_gat_prologue_backward",
                  "trx_sac_loss", "trx_sac_adam", "trx_gat_tail_infer", "trx_edge_att_weights_backward",
-                 "trx_gat_layer0_infer", "trx_gat_layer0_prepare", "trx_gat_mid_infer", "trx_partial_sum_multi"):
+                 "trx_gat_layer0_infer", "trx_gat_layer0_prepare", "trx_gat_mid_infer", "trx_partial_sum_multi",
+                 "trx_node_attention_forward", "trx_node_attention_backward", "trx_action_log_probs_forward",
+                 "trx_action_log_probs_backward", "trx_dropout_add_forward", "trx_dropout_add_backward"):
         getattr(L, name).restype = ctypes.c_int
     if L.trx_abi_version() != ABI_VERSION:
         raise ImportError(f"libtrafficrl ABI {L.trx_abi_version()} != {ABI_VERSION}")
@@ -410,6 +454,29 @@ def multi(struct_type, items):
 
 def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
+
+
+# dtype codes of the entry points that take all three
+FLOAT_CODES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+
+
+def float_code(t, what: str) -> int:
+    code = FLOAT_CODES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def on_device(what: str, first, *others):
+    """ValueError unless every tensor (None: skipped) lies on the first one's HIP
+    device; returns a context in which that device is the current one."""
+    import torch
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+    if not first.is_cuda:
+        raise ValueError(f"{what} needs tensors on a HIP device, got {first.device} (there is no CPU fallback)")
+    return torch.cuda.device(first.device)
 
 
 def stream_ptr(device=None) -> ctypes.c_void_p:

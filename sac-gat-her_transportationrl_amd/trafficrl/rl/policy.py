@@ -1,0 +1,141 @@
+"""The masked categorical policy over links as one differentiable operator
+(csrc/action_log_probs.hip): log probability of given actions, entropy and the
+best alternatives, next to DiscreteSAC's masked softmax (src/rl/sac.py:44-46)."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+
+
+class ActionLogProbs(NamedTuple):
+    log_prob: torch.Tensor                  # float32 [rows]
+    entropy: torch.Tensor                   # float32 [rows]
+    top_log_prob: Optional[torch.Tensor]    # float32 [rows, top_k]
+    top_action: Optional[torch.Tensor]      # int64 [rows, top_k]
+
+
+def _args(logits, mask, row_ptr, action, max_row, top_k, code):
+    a = _lib.TrxActionLogProbsArgs()
+    a.dtype, a.top_k = code, top_k
+    if row_ptr is None:
+        a.rows, a.row_len, a.row_stride = logits.shape[0], logits.shape[1], logits.stride(0)
+        a.mask_stride = 0 if mask is None else mask.stride(0)
+    else:
+        a.rows, a.total, a.max_row, a.row_ptr = row_ptr.numel() - 1, logits.numel(), max_row, row_ptr.data_ptr()
+    a.logits, a.action = logits.data_ptr(), action.data_ptr()
+    if mask is not None:
+        a.mask, a.mask_dtype = mask.data_ptr(), 0 if mask.dtype == torch.float32 else 1
+    return a
+
+
+def _forward(logits, mask, row_ptr, action, max_row, top_k, code):
+    L = _lib.load()
+    a = _args(logits, mask, row_ptr, action, max_row, top_k, code)
+    n, dev = a.rows, logits.device
+    log_prob = torch.empty(n, device=dev)
+    entropy = torch.empty(n, device=dev)
+    stats = torch.empty(n, 4, device=dev)
+    top_log_prob = torch.empty(n, top_k, device=dev) if top_k else None
+    top_action = torch.empty(n, top_k, device=dev, dtype=torch.int64) if top_k else None
+    a.log_prob, a.entropy, a.stats = log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
+    if top_k:
+        a.top_log_prob, a.top_action = top_log_prob.data_ptr(), top_action.data_ptr()
+    need = L.trx_action_log_probs_workspace_bytes(a)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need > 0 else None
+    a.workspace, a.workspace_bytes = 0 if ws is None else ws.data_ptr(), need
+    _lib.check(L.trx_action_log_probs_forward(a, _lib.stream_ptr(dev)), "trx_action_log_probs_forward")
+    return log_prob, entropy, top_log_prob, top_action, stats
+
+
+class _ActionLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, mask, row_ptr, action, max_row, top_k, code):
+        with torch.cuda.device(logits.device):
+            log_prob, entropy, top_log_prob, top_action, stats = _forward(logits, mask, row_ptr, action, max_row, top_k,
+                                                                          code)
+        ctx.save_for_backward(logits, mask, row_ptr, action, log_prob, entropy, stats, top_action)
+        ctx.rest = max_row, top_k, code
+        ctx.set_materialize_grads(False)
+        if top_k:
+            ctx.mark_non_differentiable(top_action)
+        return log_prob, entropy, top_log_prob, top_action
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, g_top, _g_action):
+        logits, mask, row_ptr, action, log_prob, entropy, stats, top_action = ctx.saved_tensors
+        max_row, top_k, code = ctx.rest
+        with torch.cuda.device(logits.device):
+            g = [None if t is None else t.contiguous() for t in (g_log_prob, g_entropy, g_top)]
+            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+            a = _args(logits, mask, row_ptr, action, max_row, top_k, code)
+            a.log_prob, a.entropy, a.stats = log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
+            a.top_action = 0 if top_action is None else top_action.data_ptr()
+            a.g_log_prob, a.g_entropy, a.g_top = (0 if t is None else t.data_ptr() for t in g)
+            a.grad_logits = grad.data_ptr()
+            _lib.check(_lib.load().trx_action_log_probs_backward(a, _lib.stream_ptr(logits.device)),
+                       "trx_action_log_probs_backward")
+        return grad, None, None, None, None, None, None
+
+
+def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Optional[torch.Tensor] = None,
+                     row_ptr: Optional[torch.Tensor] = None, max_row: Optional[int] = None,
+                     top_k: int = 0) -> ActionLogProbs:
+    """log softmax of each row of logits over the links that may be chosen, at
+    `action`; the row's entropy; its top_k highest log probabilities with their
+    links, highest first (ties: the lower link first).
+
+    logits: float32, bfloat16 or float16, [rows, links], or [total] with row_ptr
+    (int64 [rows + 1], each row's first link) for rows of different lengths (at
+    most 2^30 links in a row).  action: int64 [rows], row-local.  mask: shaped like
+    logits; a link may be chosen where it is > 0 (the env's action_mask; bool
+    works too).  A logit of -inf is a link that may not be chosen; large negative
+    fills are ordinary logits.  max_row: the longest row of a packed batch, a hint.
+    top_k: 0 (top_* are None) .. 16.
+
+    An action that may not be chosen, or lies outside its row, has log probability
+    -inf and passes no gradient; an empty row has entropy 0; where fewer than
+    top_k links may be chosen the rest is -inf and -1.  A row with a logit of NaN
+    or +inf that may be chosen has NaN for its values.
+
+    Differentiable once in logits through log_prob, entropy and top_log_prob.
+    Computed in float32 (the gradient rounded once to the logits' type)."""
+    what = "action_log_probs"
+    code = _lib.float_code(logits, f"{what}: logits")
+    if row_ptr is None:
+        if logits.dim() != 2:
+            raise ValueError(f"{what}: logits must be [rows, links] (or packed with row_ptr), got {tuple(logits.shape)}")
+        rows = logits.shape[0]
+    else:
+        if logits.dim() != 1:
+            raise ValueError(f"{what}: packed logits must be [total], got {tuple(logits.shape)}")
+        if row_ptr.dtype != torch.int64 or row_ptr.dim() != 1 or row_ptr.numel() < 1:
+            raise ValueError(f"{what}: row_ptr must be int64 [rows + 1]")
+        rows = row_ptr.numel() - 1
+    if action.dtype not in (torch.int64, torch.int32) or action.shape != (rows,):
+        raise ValueError(f"{what}: action must be int64 [{rows}], got {action.dtype} {tuple(action.shape)}")
+    if mask is not None and mask.shape != logits.shape:
+        raise ValueError(f"{what}: mask {tuple(mask.shape)} for logits {tuple(logits.shape)}")
+    if not 0 <= int(top_k) <= _lib.TOP_MAX:
+        raise ValueError(f"{what}: top_k must be 0..{_lib.TOP_MAX}, got {top_k}")
+    max_row = logits.numel() if max_row is None else int(max_row)
+    if max_row < 0:
+        raise ValueError(f"{what}: max_row must be >= 0")
+    max_row = min(max_row, 2 ** 30)
+    with _lib.on_device(what, logits, action, mask, row_ptr):
+        if logits.numel() and logits.stride(-1) != 1:
+            logits = logits.contiguous()
+        action = action.long().contiguous()
+        if mask is not None:
+            if mask.dtype not in (torch.float32, torch.bool, torch.uint8):
+                mask = mask > 0
+            if mask.numel() and mask.stride(-1) != 1:
+                mask = mask.contiguous()
+        row_ptr = None if row_ptr is None else row_ptr.contiguous()
+        if torch.is_grad_enabled() and logits.requires_grad:
+            return ActionLogProbs(*_ActionLogProbs.apply(logits, mask, row_ptr, action, max_row, int(top_k), code))
+        return ActionLogProbs(*_forward(logits, mask, row_ptr, action, max_row, int(top_k), code)[:4])

@@ -30,6 +30,7 @@ import torch.nn.functional as F
 from ..models import fused
 from ..models.gat_encoder import GATEncoder, is_regular_batch
 from ..models.skinny import regular_gather, skinny_linear, splitk_linear
+from .policy import ActionLogProbs, action_log_probs
 
 
 @dataclass
@@ -432,6 +433,17 @@ class DiscreteSAC:
         if deterministic:
             return p.argmax(dim=1)
         return torch.multinomial(p, 1, generator=generator).squeeze(1)
+
+    def evaluate_actions(self, node_x, edge_index, edge_attr, action_mask, batch, num_graphs: int, actions,
+                         top_k: int = 0) -> ActionLogProbs:
+        """Log probabilities of given actions (one per graph, link ids), the
+        policy's entropy and its top_k best alternatives, for B graphs with
+        identical link counts; differentiable in the actor's parameters where
+        gradients are enabled (imitation losses, probability ratios)."""
+        with self._amp():
+            logits, _, _ = self.actor(node_x, edge_index, edge_attr, action_mask, batch, num_graphs=num_graphs)
+        return action_log_probs(logits.view(num_graphs, -1), actions, mask=action_mask.view(num_graphs, -1),
+                                top_k=top_k)
 
     # ------------------------------------------------------------ update
     def update(self, batch, weights=None, alpha_max: float = None, sync_metrics: bool = True):
