@@ -1339,7 +1339,8 @@ int check_attention_shape(const trx_node_attention_args* a) {
                     TRX_ATT_MAX_CHANNELS, a->channels);
     if (a->num_queries > (int64_t(1) << 31) - 1 || a->num_nodes > (int64_t(1) << 31) - 1)
         return fail(TRX_EUNSUP, "node_attention: at most 2^31 - 1 rows");
-    if (a->num_graphs > (1 << 24)) return fail(TRX_EUNSUP, "node_attention: at most 2^24 graphs");
+    if ((int64_t)a->num_graphs + 1 > (1 << 23) / a->heads)
+        return fail(TRX_EUNSUP, "node_attention: at most 2^23 / heads graphs");
     return TRX_OK;
 }
 

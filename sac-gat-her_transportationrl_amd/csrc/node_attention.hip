@@ -1,257 +1,284 @@
 // node_attention.hip -- softmax attention of query rows over the nodes of their
-// own network (include/trafficrl.h, trx_node_attention_*): scores scaled,
-// optionally capped by a tanh, lowered by slope[h] times the pair's distance,
-// pairs at no finite distance unseen.
+// own network, forward (include/trafficrl.h, trx_node_attention_*; backward:
+// node_attention_bwd.hip): scores scaled, optionally capped by a tanh, lowered
+// by slope[h] times the pair's distance, pairs at no finite distance unseen.
 //
-// Forward: one wave per (query row, head), its lanes over the channels, one
-// pass over the keys with the running maximum and sum.  Backward: one wave per
-// (query row, head) for grad_q and the slope, one per (node, kv head) for
-// grad_k and grad_v; the probabilities come back from the saved lse.
-#include <hip/hip_runtime.h>
+// One pass over a graph's keys with the running maximum and sum of the softmax.
+// A workgroup holds WAVES x 16 MQ rows of one (graph, key/value head): the
+// query rows of all heads that share the key/value head, row-major (query, head
+// of the group), so a shared head's keys are read once.  Keys and values pass
+// through LDS in tiles of KT, the next tile on its way in registers.
+#include <algorithm>
 
-#include "float_types.h"
-#include "trx_internal.h"
+#include "node_attention.h"
 
 namespace trx {
 namespace {
 
-constexpr int kWave = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
-
-using Args = trx_node_attention_args;
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-struct Span {
-    int64_t at;
-    int n;
-};
-
-// graph b's rows, clamped to the tensor; graph num_graphs: none
-__device__ __forceinline__ Span span(const int64_t* ptr, int b, int64_t rows) {
-    int64_t lo = ptr[b], hi = ptr[b + 1];
-    lo = lo < 0 ? 0 : lo > rows ? rows : lo;
-    hi = hi < lo ? lo : hi > rows ? rows : hi;
-    return {lo, (int)(hi - lo)};
-}
-
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
-
-// the distance of pair (i, j) of graph b, +inf where the pair is not seen
-__device__ __forceinline__ float distance(const Args& a, int b, int i, int j) {
-    if (!a.dist) return 0.0f;
-    if (i >= a.dist_rows || j >= a.dist_cols) return INFINITY;
-    const float d = a.dist[b * a.dist_graph + i * a.dist_row + j];
-    return finite(d) ? d : INFINITY;
-}
-
-// rows of no graph: before the first and behind the last
-template <typename T>
-__device__ __forceinline__ void zero_rest(T* out, const int64_t* ptr, int graphs, int64_t rows, int64_t width, int at,
-                                          int step) {
-    if (!out) return;
-    int64_t begin = graphs > 0 ? ptr[0] : 0, end = graphs > 0 ? ptr[graphs] : 0;
-    begin = begin < 0 ? 0 : begin > rows ? rows : begin;
-    end = end < begin ? begin : end > rows ? rows : end;
-    for (int64_t e = at; e < begin * width; e += step) out[e] = (T)0.0f;
-    for (int64_t e = end * width + at; e < rows * width; e += step) out[e] = (T)0.0f;
-}
-
-struct Score {
-    float w, slack, d;   // the biased score in units of log 2, dz/d(scaled product), the distance
-    bool seen;
-};
-__device__ __forceinline__ Score score(const Args& a, float dot, float d, float slope) {
-    float z = dot * a.scale, slack = 1.0f;
-    if (a.cap > 0.0f) {
-        const float t = tanhf(z / a.cap);
-        z = a.cap * t;
-        slack = 1.0f - t * t;
-    }
-    if (!finite(d)) return {-INFINITY, 0.0f, 0.0f, false};
-    return {(z - slope * d) * kLog2e, slack, d, true};
-}
-
-template <typename T>
-__device__ __forceinline__ float2 two(const T* row, int C, int lane) {
-    return {lane < C ? (float)row[lane] : 0.0f, lane + kWave < C ? (float)row[lane + kWave] : 0.0f};
-}
-template <typename T>
-__device__ __forceinline__ void put(T* row, int C, int lane, float x, float y) {
-    if (lane < C) row[lane] = (T)x;
-    if (lane + kWave < C) row[lane + kWave] = (T)y;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kWave) attention_fwd_kernel(Args a) {
-    const int lane = threadIdx.x, b = blockIdx.x, h = blockIdx.z, C = a.channels;
+template <typename T, int CP, int MQ, int WAVES, int KT>
+__global__ void __launch_bounds__(kWave* WAVES) attention_fwd_kernel(Args a, float* part) {
+    constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
+    __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
+    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
+    const int b = blockIdx.x / a.kv_heads, hk = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads, C = a.channels;
     T* out = static_cast<T*>(a.out);
     if (b == a.num_graphs) {
-        const int at = (blockIdx.z * gridDim.y + blockIdx.y) * kWave + lane, step = gridDim.y * gridDim.z * kWave;
-        zero_rest(out, a.q_ptr, b, a.num_queries, (int64_t)a.heads * C, at, step);
+        if (!part && hk == 0)
+            zero_rest(out, a.q_ptr, b, a.num_queries, (int64_t)a.heads * C, blockIdx.y * kThreads + threadIdx.x,
+                      gridDim.y * kThreads);
         return;
     }
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
-    const int hk = h / (a.heads / a.kv_heads);
-    const float slope = a.slope ? a.slope[h] : 0.0f;
-    for (int i = blockIdx.y; i < qs.n; i += gridDim.y) {
-        const int64_t row = qs.at + i;
-        const float2 q = two(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head, C, lane);
-        float m = -INFINITY, l = 0.0f, ox = 0.0f, oy = 0.0f;
-        for (int j = 0; j < ks.n; ++j) {
-            const float2 k = two(static_cast<const T*>(a.k) + (ks.at + j) * a.k_row + hk * a.k_head, C, lane);
-            const Score s = score(a, wave_sum(q.x * k.x + q.y * k.y), distance(a, b, i, j), slope);
-            if (s.w == -INFINITY) continue;
-            const float2 v = two(static_cast<const T*>(a.v) + (ks.at + j) * a.v_row + hk * a.v_head, C, lane);
-            const float mn = s.w > m ? s.w : m, f = exp2f(m - mn), p = exp2f(s.w - mn);
-            l = l * f + p;
-            ox = ox * f + p * v.x;
-            oy = oy * f + p * v.y;
-            m = mn;
-        }
-        const float r = l == 0.0f ? 0.0f : 1.0f / l;
-        put(out + (row * a.heads + h) * C, C, lane, ox * r, oy * r);
-        if (a.lse && lane == 0) a.lse[row * a.heads + h] = l == 0.0f ? -INFINITY : m + log2f(l);
-    }
-}
+    const int64_t rows = (int64_t)qs.n * G;
+    const int keys_each = ((ks.n + KT - 1) / KT + gridDim.z - 1) / gridDim.z * KT;
+    const int first = min((int64_t)ks.n, (int64_t)blockIdx.z * keys_each), last = min(ks.n, first + keys_each);
+    const T* k_base = static_cast<const T*>(a.k) + ks.at * a.k_row + hk * a.k_head;
+    const T* v_base = static_cast<const T*>(a.v) + ks.at * a.v_row + hk * a.v_head;
+    const float mul = a.cap > 0.0f ? a.scale / a.cap : a.scale;
 
-template <typename T>
-__global__ void __launch_bounds__(kWave) attention_bwd_q_kernel(Args a, float* dots, float* slopes) {
-    const int lane = threadIdx.x, b = blockIdx.x, h = blockIdx.z, C = a.channels;
-    const int at = (blockIdx.z * gridDim.y + blockIdx.y) * kWave + lane, step = gridDim.y * gridDim.z * kWave;
-    T* gq = static_cast<T*>(a.grad_q);
-    if (b == a.num_graphs) {
-        zero_rest(gq, a.q_ptr, b, a.num_queries, (int64_t)a.heads * C, at, step);
-        zero_rest(slopes, a.q_ptr, b, a.num_queries, (int64_t)a.heads, at, step);
-        return;
-    }
-    const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
-    const int hk = h / (a.heads / a.kv_heads);
-    const float slope = a.slope ? a.slope[h] : 0.0f;
-    for (int i = blockIdx.y; i < qs.n; i += gridDim.y) {
-        const int64_t row = qs.at + i, o = row * a.heads + h;
-        const float2 q = two(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head, C, lane);
-        const float2 go = two(static_cast<const T*>(a.grad_out) + o * C, C, lane);
-        const float2 ov = two(static_cast<const T*>(a.out) + o * C, C, lane);
-        const float D = wave_sum(go.x * ov.x + go.y * ov.y), lse = a.lse[o];
-        float gx = 0.0f, gy = 0.0f, pd = 0.0f, u = 0.0f, ud = 0.0f;
-        for (int j = 0; j < ks.n && lse > -INFINITY; ++j) {
-            const float2 k = two(static_cast<const T*>(a.k) + (ks.at + j) * a.k_row + hk * a.k_head, C, lane);
-            const float2 v = two(static_cast<const T*>(a.v) + (ks.at + j) * a.v_row + hk * a.v_head, C, lane);
-            const Score s = score(a, wave_sum(q.x * k.x + q.y * k.y), distance(a, b, i, j), slope);
-            if (s.w == -INFINITY) continue;
-            const float p = exp2f(s.w - lse), gp = wave_sum(go.x * v.x + go.y * v.y);
-            const float w = p * (gp - D), t = w * s.slack * a.scale;
-            gx += t * k.x;
-            gy += t * k.y;
-            pd += p * s.d;
-            u += w;
-            ud += w * s.d;
+    for (int64_t tile = blockIdx.y; tile * kRows < rows; tile += gridDim.y) {
+        const int64_t row0 = tile * kRows + w * 16 * MQ;
+        frag<T> q[MQ][kSteps];
+        const float* dist[MQ];
+        float slope[MQ], m[MQ], l[MQ];
+        int limit[MQ];
+        f32x4 o[MQ][CP / 16];
+#pragma unroll
+        for (int t = 0; t < MQ; ++t) {
+            const int64_t row = min(row0 + 16 * t + c, rows - 1);
+            const int i = (int)(row / G), h = hk * G + (int)(row % G);
+            const T* p = static_cast<const T*>(a.q) + (qs.at + i) * a.q_row + h * a.q_head;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[t][s] = 32 * s + 8 * g < C ? load_frag(p + 32 * s + 8 * g) : zero_frag<T>();
+            slope[t] = a.slope ? -a.slope[h] : 0.0f;
+            dist[t] = a.dist ? a.dist + b * a.dist_graph + i * a.dist_row : nullptr;
+            limit[t] = !a.dist ? ks.n : i < a.dist_rows ? min(ks.n, a.dist_cols) : 0;
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < CP / 16; ++x) o[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        put(gq + o * C, C, lane, gx, gy);
-        if (lane == 0) {
-            dots[o] = D;
-            slopes[o] = u * pd - ud;   // D stands on the rounded out: what is left of sum w corrects it
+        Staged<T, CP, KT, kThreads> k_next, v_next;
+        auto fetch = [&](int j0) {
+            k_next.load(C, [&](int j) { return j0 + j < ks.n ? k_base + (j0 + j) * a.k_row : nullptr; });
+            v_next.load(C, [&](int j) { return j0 + j < ks.n ? v_base + (j0 + j) * a.v_row : nullptr; });
+        };
+        if (first < last) fetch(first);
+        for (int j0 = first; j0 < last; j0 += KT) {
+            __syncthreads();
+            k_next.store(k_tile);
+            v_next.store(v_tile);
+            __syncthreads();
+            if (j0 + KT < last) fetch(j0 + KT);
+            if (row0 >= rows) continue;
+            f32x4 d[MQ][kTiles];
+            if (a.dist) {
+#pragma unroll
+                for (int t = 0; t < MQ; ++t) {
+                    const bool whole = __all(j0 + KT <= limit[t]);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) d[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
+                }
+            }
+            f32x4 s[MQ][kTiles];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+                for (int t = 0; t < MQ; ++t) s[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < kSteps; ++x) {
+                    const frag<T> f = load_frag(k_tile + (16 * n + c) * kRow<T, CP> + 32 * x + 8 * g);
+#pragma unroll
+                    for (int t = 0; t < MQ; ++t) s[t][n] = mma(f, q[t][x], s[t][n]);
+                }
+            }
+            frag<T> p[MQ][KT / 32];
+#pragma unroll
+            for (int t = 0; t < MQ; ++t) {
+                // scores, and their maximum
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][n][r] = a.cap * tanh_of<T>(s[t][n][r], mul);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) s[t][n] = s[t][n] * mul;
+                }
+                if (a.dist) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            s[t][n][r] = finite(d[t][n][r]) ? __builtin_fmaf(slope[t], d[t][n][r], s[t][n][r]) : -INFINITY;
+                } else if (j0 + KT > ks.n) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j0 + 16 * n + 4 * g + r >= ks.n) s[t][n][r] = -INFINITY;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][n][r]);
+                top = column_max(top);
+                // The reference point moves only when a score passes it by 5.5, a factor of 2^8 in the sums: nothing
+                // is lost in float32, and the accumulators are rescaled once or twice a row instead of at every new
+                // maximum.
+                const bool move = top > m[t] + 5.5f;
+                if (__any(move)) {
+                    const float f = move ? exp2_fast((m[t] - top) * kLog2e) : 1.0f;
+                    m[t] = move ? top : m[t];
+                    l[t] *= f;
+#pragma unroll
+                    for (int x = 0; x < CP / 16; ++x) o[t][x] = o[t][x] * f;
+                }
+                const float base = m[t] == -INFINITY ? 0.0f : -m[t] * kLog2e;
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = exp2_fast(__builtin_fmaf(s[t][n][r], kLog2e, base));
+                        l[t] += e;
+                        p[t][n / 2][4 * (n % 2) + r] = (T)e;   // rounded to the type for the product with v
+                    }
+            }
+#pragma unroll
+            for (int x = 0; x < CP / 16; ++x)
+#pragma unroll
+                for (int u = 0; u < KT / 32; ++u) {
+                    const frag<T> f = turned<T, CP>(v_tile, 32 * u, 32 * u + 16, 16 * x, lane);
+#pragma unroll
+                    for (int t = 0; t < MQ; ++t) o[t][x] = mma(f, p[t][u], o[t][x]);
+                }
         }
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kWave) attention_bwd_kv_kernel(Args a, const float* dots) {
-    const int lane = threadIdx.x, b = blockIdx.x, hk = blockIdx.z, C = a.channels;
-    const int at = (blockIdx.z * gridDim.y + blockIdx.y) * kWave + lane, step = gridDim.y * gridDim.z * kWave;
-    T *gk = static_cast<T*>(a.grad_k), *gv = static_cast<T*>(a.grad_v);
-    if (b == a.num_graphs) {
-        zero_rest(gk, a.k_ptr, b, a.num_nodes, (int64_t)a.kv_heads * C, at, step);
-        zero_rest(gv, a.k_ptr, b, a.num_nodes, (int64_t)a.kv_heads * C, at, step);
-        return;
-    }
-    const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
-    const int G = a.heads / a.kv_heads;
-    for (int j = blockIdx.y; j < ks.n; j += gridDim.y) {
-        const float2 k = two(static_cast<const T*>(a.k) + (ks.at + j) * a.k_row + hk * a.k_head, C, lane);
-        const float2 v = two(static_cast<const T*>(a.v) + (ks.at + j) * a.v_row + hk * a.v_head, C, lane);
-        float kx = 0.0f, ky = 0.0f, vx = 0.0f, vy = 0.0f;
-        for (int i = 0; i < qs.n; ++i) {
-            const float d = distance(a, b, i, j);
-            if (!finite(d)) continue;
-            for (int h = hk * G; h < hk * G + G; ++h) {
-                const int64_t row = qs.at + i, o = row * a.heads + h;
-                const float lse = a.lse[o];
-                const float2 q = two(static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head, C, lane);
-                const float2 go = two(static_cast<const T*>(a.grad_out) + o * C, C, lane);
-                const Score s = score(a, wave_sum(q.x * k.x + q.y * k.y), d, a.slope ? a.slope[h] : 0.0f);
-                if (s.w == -INFINITY || lse == -INFINITY) continue;
-                const float p = exp2f(s.w - lse), gp = wave_sum(go.x * v.x + go.y * v.y);
-                const float t = p * (gp - dots[o]) * s.slack * a.scale;
-                kx += t * q.x;
-                ky += t * q.y;
-                vx += p * go.x;
-                vy += p * go.y;
+#pragma unroll
+        for (int t = 0; t < MQ; ++t) {
+            const float sum = column_sum(l[t]);
+            const int64_t row = row0 + 16 * t + c;
+            if (row >= rows) continue;
+            const int i = (int)(row / G), h = hk * G + (int)(row % G);
+            const int64_t at = (qs.at + i) * a.heads + h;
+            if (part) {   // this split's sum and accumulator, for join_kernel
+                const int64_t all = a.num_queries * a.heads, mine = blockIdx.z * all + at;
+                float* stat = part + (int64_t)gridDim.z * all * C;
+                if (g == 0) {
+                    stat[2 * mine] = m[t] * kLog2e;
+                    stat[2 * mine + 1] = sum;
+                }
+#pragma unroll
+                for (int x = 0; x < CP / 16; ++x)
+                    if (16 * x + 4 * g < C) *reinterpret_cast<f32x4*>(part + mine * C + 16 * x + 4 * g) = o[t][x];
+            } else {
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (a.lse && g == 0) a.lse[at] = sum == 0.0f ? -INFINITY : m[t] * kLog2e + log2f(sum);
+#pragma unroll
+                for (int x = 0; x < CP / 16; ++x)
+                    if (16 * x + 4 * g < C) {
+                        typedef T T4 __attribute__((ext_vector_type(4)));
+                        T4 y;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) y[r] = (T)(o[t][x][r] * f);
+                        *reinterpret_cast<T4*>(out + at * C + 16 * x + 4 * g) = y;
+                    }
             }
         }
-        const int64_t o = (ks.at + j) * a.kv_heads + hk;
-        put(gk + o * C, C, lane, kx, ky);
-        put(gv + o * C, C, lane, vx, vy);
     }
 }
 
-// grad_slope[h] = the sum of its column, in a fixed order: 16 waves over the rows, lanes over their rows
-__global__ void __launch_bounds__(kWave * 16) slope_sum_kernel(const float* slopes, int64_t rows, int heads, float* out) {
-    __shared__ float part[16];
-    const int h = blockIdx.x, lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave;
-    float v = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += kWave * 16) v += slopes[r * heads + h];
-    v = wave_sum(v);
-    if (lane == 0) part[w] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; ++k) v += part[k];
-        out[h] = v;
+// out and lse from the splits' sums: one wave per (row, head), rows of no graph zero
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_kernel(Args a, const float* part, int splits) {
+    const int lane = threadIdx.x % kWave;
+    const int64_t all = a.num_queries * a.heads, at = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    if (at >= all) return;
+    const Span qs = all_rows(a.q_ptr, a.num_graphs, a.num_queries);
+    const int64_t row = at / a.heads;
+    T* out = static_cast<T*>(a.out) + at * a.channels;
+    const float* stat = part + splits * all * a.channels;
+    float m = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+    if (row >= qs.at && row < qs.at + qs.n) {
+        for (int s = 0; s < splits; ++s) m = fmaxf(m, stat[2 * (s * all + at)]);
+        for (int s = 0; s < splits; ++s) {
+            const int64_t mine = s * all + at;
+            const float f = stat[2 * mine] == -INFINITY ? 0.0f : exp2_fast(stat[2 * mine] - m);
+            // a split without a finite score adds its sum as it is: zero, or the NaN that it saw
+            l += stat[2 * mine] == -INFINITY ? stat[2 * mine + 1] : stat[2 * mine + 1] * f;
+            if (lane < a.channels) x += part[mine * a.channels + lane] * f;
+            if (lane + kWave < a.channels) y += part[mine * a.channels + lane + kWave] * f;
+        }
+        if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : m + log2f(l);
     }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    if (lane < a.channels) out[lane] = (T)(x * f);
+    if (lane + kWave < a.channels) out[lane + kWave] = (T)(y * f);
 }
 
-unsigned rows_of(int64_t most, int64_t rows) {
-    const int64_t n = most < rows ? most : rows;
-    return (unsigned)(n < 1 ? 1 : n > 4096 ? 4096 : n);
+// How a forward pass is cut.  Up to 32 rows to a (graph, head), one wave has them all and a workgroup of more would
+// idle; else four waves share each tile of keys.  Keys are split where the rows alone leave most of the 256 compute
+// units without a workgroup, into pieces of at least 256 keys (a piece costs its accumulator's round trip).
+struct Cut {
+    bool narrow;   // one wave
+    int mq;        // 16-row tiles of a wave
+    int64_t tiles;
+    int splits;
+};
+Cut cut_fwd(const Args& a) {
+    const int64_t G = a.heads / a.kv_heads, units = (int64_t)a.num_graphs * a.kv_heads;
+    const int64_t rows = std::min(a.max_queries, a.num_queries) * G, keys = std::min(a.max_nodes, a.num_nodes);
+    Cut c;
+    c.narrow = rows <= 32;
+    c.mq = c.narrow && rows <= 16 ? 1 : 2;
+    const int64_t each = c.narrow ? 16 * c.mq : 128;
+    c.tiles = std::max<int64_t>(1, std::min<int64_t>((rows + each - 1) / each, 65535));
+    const int64_t blocks = std::max<int64_t>(1, units * c.tiles), want = c.narrow ? 2048 : 512;
+    const int64_t most = std::min<int64_t>(64, std::min(keys / 256, (int64_t(1) << 28) / std::max<int64_t>(1, a.num_queries * a.heads * (a.channels + 2) * 4)));
+    c.splits = (int)std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, most));
+    return c;
 }
 
 }  // namespace
 
 size_t node_attention_workspace(const trx_node_attention_args& a, bool backward) {
-    return backward ? (size_t)a.num_queries * a.heads * 2 * sizeof(float) : 0;
+    if (backward) return attention_bwd_workspace(a);
+    const int splits = cut_fwd(a).splits;
+    return splits > 1 ? (size_t)splits * a.num_queries * a.heads * (a.channels + 2) * sizeof(float) : 0;
+}
+
+template <typename T, int CP>
+static void launch_fwd(const Args& a, const Cut& c, hipStream_t stream) {
+    float* part = c.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
+    const dim3 grid((unsigned)((a.num_graphs + 1) * (int64_t)a.kv_heads), (unsigned)c.tiles, c.splits);
+    constexpr int kWide = sizeof(T) == 2 ? 64 : 32;
+    if (!c.narrow)
+        hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 2, 4, kWide>), grid, dim3(256), 0, stream, a, part);
+    else if (c.mq == 2)
+        hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 2, 1, 32>), grid, dim3(64), 0, stream, a, part);
+    else
+        hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 1, 1, 32>), grid, dim3(64), 0, stream, a, part);
+    if (part)
+        hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)((a.num_queries * a.heads + 3) / 4)), dim3(256), 0,
+                           stream, a, part, c.splits);
 }
 
 hipError_t launch_node_attention_fwd(const trx_node_attention_args& a, hipStream_t stream) {
+    const Cut c = cut_fwd(a);
     return by_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const dim3 grid(a.num_graphs + 1, rows_of(a.max_queries, a.num_queries), a.heads);
-        hipLaunchKernelGGL(attention_fwd_kernel<T>, grid, dim3(kWave), 0, stream, a);
+        if (a.channels <= 32)
+            launch_fwd<T, 32>(a, c, stream);
+        else if (a.channels <= 64)
+            launch_fwd<T, 64>(a, c, stream);
+        else
+            launch_fwd<T, 128>(a, c, stream);
         return hipGetLastError();
     });
 }
 
 hipError_t launch_node_attention_bwd(const trx_node_attention_args& a, hipStream_t stream) {
-    float *dots = static_cast<float*>(a.workspace), *slopes = dots + a.num_queries * a.heads;
-    return by_dtype(a.dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        if (a.num_queries > 0) {
-            const dim3 grid(a.num_graphs + 1, rows_of(a.max_queries, a.num_queries), a.heads);
-            hipLaunchKernelGGL(attention_bwd_q_kernel<T>, grid, dim3(kWave), 0, stream, a, dots, slopes);
-        }
-        if (a.num_nodes > 0) {
-            const dim3 grid(a.num_graphs + 1, rows_of(a.max_nodes, a.num_nodes), a.kv_heads);
-            hipLaunchKernelGGL(attention_bwd_kv_kernel<T>, grid, dim3(kWave), 0, stream, a, dots);
-        }
-        if (a.grad_slope)
-            hipLaunchKernelGGL(slope_sum_kernel, dim3(a.heads), dim3(kWave * 16), 0, stream, slopes, a.num_queries,
-                               a.heads, a.grad_slope);
-        return hipGetLastError();
-    });
+    return launch_attention_bwd(a, stream);
 }
 
 }  // namespace trx
