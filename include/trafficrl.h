@@ -878,7 +878,9 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
  * grad_q [num_queries, heads, channels], grad_k, grad_v [num_nodes, kv_heads,
  * channels]: contiguous, in dtype.  lse float32 [num_queries, heads]:
  * log2(sum_j 2^(w log2 e)), written by the forward where not NULL (-inf for an
- * empty row), read by the backward.  grad_slope float32 [heads] or NULL.
+ * empty row), read by the backward.  out_low: like out, or NULL: what rounding
+ * took from out; with it the backward's <grad_out, out> is as exact as in
+ * float32.  grad_slope float32 [heads] or NULL.
  * max_queries / max_nodes: the largest graph's rows; they only shape the
  * launch (a smaller value costs time, never rows).  Sums and the softmax's
  * statistics are float32; probabilities and score gradients enter the matrix
@@ -897,7 +899,7 @@ typedef struct trx_node_attention_args {
     const float* dist;
     int64_t dist_graph, dist_row;
     const float* slope;                 /* [heads] */
-    void* out;
+    void *out, *out_low;
     float* lse;
     const void* grad_out;
     void *grad_q, *grad_k, *grad_v;

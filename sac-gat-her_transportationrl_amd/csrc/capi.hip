@@ -1337,6 +1337,8 @@ int check_attention_shape(const trx_node_attention_args* a) {
     if (a->channels < 8 || a->channels > TRX_ATT_MAX_CHANNELS || a->channels % 8 != 0)
         return fail(TRX_EUNSUP, "node_attention: channels must be a multiple of 8 up to %d (got %d)",
                     TRX_ATT_MAX_CHANNELS, a->channels);
+    if (a->num_queries > ((int64_t(1) << 31) - 256) / (a->heads / a->kv_heads))
+        return fail(TRX_EUNSUP, "node_attention: query rows x heads of a group must stay below 2^31 - 256");
     if (a->num_queries > (int64_t(1) << 31) - 1 || a->num_nodes > (int64_t(1) << 31) - 1)
         return fail(TRX_EUNSUP, "node_attention: at most 2^31 - 1 rows");
     if ((int64_t)a->num_graphs + 1 > (1 << 23) / a->heads)
@@ -1356,7 +1358,7 @@ int check_attention(const trx_node_attention_args* a, bool backward) {
     for (int64_t s : {a->q_row, a->q_head, a->k_row, a->k_head, a->v_row, a->v_head})
         if (s < 0 || s % unit != 0)
             return fail(TRX_EINVAL, "node_attention: strides must be multiples of 16 bytes and not negative");
-    for (const void* p : {a->q, a->k, a->v, (const void*)a->out, a->grad_out, (const void*)a->grad_q,
+    for (const void* p : {a->q, a->k, a->v, (const void*)a->out, (const void*)a->out_low, a->grad_out, (const void*)a->grad_q,
                           (const void*)a->grad_k, (const void*)a->grad_v, (const void*)a->workspace})
         if (misaligned(p)) return fail(TRX_EINVAL, "node_attention: buffers must be 16-byte aligned");
     if (a->dist && (a->dist_rows < 0 || a->dist_cols < 0 || a->dist_row < 0 || a->dist_graph < 0))

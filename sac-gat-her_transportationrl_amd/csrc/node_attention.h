@@ -16,6 +16,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "float_types.h"
 #include "trx_internal.h"
 
@@ -97,31 +99,97 @@ __device__ __forceinline__ frag<T> turned(const T* tile, int row0, int row1, int
     }
 }
 
-// ROWS x CP elements on their way from memory to LDS through registers: loaded
-// while the tile before is worked on
+// ROWS x CP elements of consecutive rows on their way from memory to LDS through
+// registers: loaded while the tile before is worked on
 template <typename T, int CP, int ROWS, int THREADS>
 struct Staged {
     static constexpr int kChunks = ROWS * (CP / 8), kEach = (kChunks + THREADS - 1) / THREADS;
     Eight<T> r[kEach];
+    const T* p[kEach];
 
-    // row(i) -> pointer to row i's first element, or null where there is none
-    template <typename F>
-    __device__ __forceinline__ void load(int C, F&& row) {
+    static __device__ __forceinline__ int row_of(int e) { return (threadIdx.x + e * THREADS) / (CP / 8); }
+    static __device__ __forceinline__ int channel_of(int e) { return 8 * ((threadIdx.x + e * THREADS) % (CP / 8)); }
+
+    __device__ __forceinline__ void start(const T* first, int64_t row) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) p[e] = first + row_of(e) * row + channel_of(e);
+    }
+    // `left` rows are there; step: ROWS rows on
+    __device__ __forceinline__ void load(int C, int left, int64_t step) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int x = threadIdx.x + e * THREADS, i = x / (CP / 8), c = 8 * (x % (CP / 8));
-            const T* p = x < kChunks ? row(i) : nullptr;
-            r[e] = p && c < C ? load8(p + c) : Eight<T>{};
+            const bool in = row_of(e) < left && row_of(e) < ROWS && channel_of(e) < C;
+            r[e] = in ? load8(p[e]) : Eight<T>{};
+            p[e] += step;
+        }
+    }
+    // the same with a pointer of its own for each row
+    template <typename F>
+    __device__ __forceinline__ void load_rows(int C, int left, F&& row) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const bool in = row_of(e) < left && row_of(e) < ROWS && channel_of(e) < C;
+            r[e] = in ? load8(row(row_of(e)) + channel_of(e)) : Eight<T>{};
         }
     }
     __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int x = threadIdx.x + e * THREADS, i = x / (CP / 8), c = 8 * (x % (CP / 8));
-            if (x < kChunks) store8(tile + i * kRow<T, CP> + c, r[e]);
-        }
+        for (int e = 0; e < kEach; ++e)
+            if (kChunks % THREADS == 0 || row_of(e) < ROWS) store8(tile + row_of(e) * kRow<T, CP> + channel_of(e), r[e]);
     }
 };
+
+// n / d for 0 <= n < 2^31 by a multiplication
+struct Divide {
+    uint32_t mul, shift, by;
+    __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
+inline Divide divide_by(int d) {
+    uint32_t s = 0;
+    while ((int64_t(1) << s) < d) ++s;
+    return {(uint32_t)((uint64_t(1) << (31 + s)) / d + 1), 31 + s, (uint32_t)d};
+}
+
+// the arguments of a launch
+struct Call {
+    Args a;
+    Divide group, kv;   // by heads of a group, by key/value heads
+};
+inline Call call_of(const Args& a) { return {a, divide_by(a.heads / a.kv_heads), divide_by(a.kv_heads)}; }
+
+// four elements of a result; where `low` is given, what rounding took from them goes there
+template <typename T>
+__device__ __forceinline__ void put4(T* out, T* low, int64_t at, f32x4 v) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (T)v[r];
+    *reinterpret_cast<T4*>(out + at) = y;
+    if (low) {
+        T4 z;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = (T)(v[r] - (float)y[r]);
+        *reinterpret_cast<T4*>(low + at) = z;
+    }
+}
+
+// 16-row tiles of a wave in a workgroup of four: two, one where float32's accumulators and operands of 128 channels
+// would not leave registers for two waves
+template <typename T, int CP>
+constexpr int kTilesOfWave = sizeof(T) == 4 && CP == 128 ? 1 : 2;
+
+// calls f with the padded channels, whether there are distances, whether scores are capped
+template <typename T, typename F>
+inline hipError_t by_shape(const Args& a, F&& f) {
+    auto second = [&](auto cp) {
+        if (a.dist)
+            return a.cap > 0.0f ? f(cp, std::true_type{}, std::true_type{}) : f(cp, std::true_type{}, std::false_type{});
+        return a.cap > 0.0f ? f(cp, std::false_type{}, std::true_type{}) : f(cp, std::false_type{}, std::false_type{});
+    };
+    if (a.channels <= 32) return second(std::integral_constant<int, 32>{});
+    if (a.channels <= 64) return second(std::integral_constant<int, 64>{});
+    return second(std::integral_constant<int, 128>{});
+}
 
 struct Span {
     int64_t at;
@@ -175,6 +243,37 @@ __device__ __forceinline__ float column_max(float v) {
     return fmaxf(v, __shfl_xor(v, 32));
 }
 
+// Scores w = scale x - slope d, unseen at -inf.  Where every lane's slope is
+// positive and the scale too (`plain`), they are kept divided by the scale: the
+// product with it joins the exponential's, and a distance of +inf makes its -inf
+// by itself, so one multiply-add a score is all.  Distances that are negative or
+// NaN anywhere in the tile, or other signs, take selects.
+struct Bias {
+    float slope;   // -slope / scale where plain, else -slope
+    float pre;     // what scores are multiplied by first
+    float unit;    // from the scores' unit to log 2
+    bool plain;
+};
+template <bool DIST, bool CAP>
+__device__ __forceinline__ Bias bias_of(const Args& a, float slope) {
+    Bias b;
+    b.plain = !CAP && a.scale > 1e-18f;
+    if (DIST) b.plain = b.plain && __all(slope > 0.0f && slope < 1e18f);
+    b.pre = CAP ? a.scale / a.cap : b.plain ? 1.0f : a.scale;
+    b.slope = b.plain ? -slope / a.scale : -slope;
+    b.unit = b.plain ? a.scale * kLog2e : kLog2e;
+    return b;
+}
+template <int N>
+__device__ __forceinline__ bool ordinary(const f32x4 (&d)[N]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(d[n][r]));
+    return __all(most <= 0x7f800000u);   // neither negative nor NaN
+}
+
 // one column's four distances behind key j: +inf from `limit` on
 __device__ __forceinline__ f32x4 distances(const float* row, int j, int limit, bool whole) {
     if (whole) return *reinterpret_cast<const f32x4u*>(row + j);
@@ -186,8 +285,23 @@ __device__ __forceinline__ f32x4 distances(const float* row, int j, int limit, b
 
 }  // namespace
 
-// node_attention_bwd.hip
+// How a pass over kept rows (grid.y tiles of them) and an axis that is run over
+// (grid.z splits of it) is cut
+struct AttentionCut {
+    bool narrow;   // one wave
+    int mq;        // its 16-row tiles
+    int64_t tiles;
+    int splits;
+};
+// node_attention_fwd.h, node_attention_bwd.h; instantiated in node_attention_{f32,bf16,f16}.hip
+template <typename T>
+hipError_t launch_attention_fwd(const trx_node_attention_args& a, hipStream_t stream);
+template <typename T>
 hipError_t launch_attention_bwd(const trx_node_attention_args& a, hipStream_t stream);
-size_t attention_bwd_workspace(const trx_node_attention_args& a);
+AttentionCut cut_fwd(const trx_node_attention_args& a);
+AttentionCut cut_bwd_q(const trx_node_attention_args& a);
+AttentionCut cut_bwd_kv(const trx_node_attention_args& a);
+size_t attention_row_floats(const trx_node_attention_args& a);
+constexpr int kSlopeChunks = 64;   // of the rows, each with its own sum of the slopes' gradients
 
 }  // namespace trx

@@ -1,0 +1,259 @@
+// node_attention_fwd.h -- node_attention's forward kernels, one element type to
+// a translation unit (node_attention_{f32,bf16,f16}.hip).
+//
+// One pass over a graph's keys with the running maximum and sum of the softmax.
+// A workgroup holds WAVES x 16 MQ rows of one (graph, key/value head): the
+// query rows of all heads that share the key/value head, row-major (query, head
+// of the group), so a shared head's keys are read once.  Keys and values pass
+// through LDS in tiles of KT, the next tile on its way in registers.
+#pragma once
+#include <algorithm>
+
+#include "node_attention.h"
+
+namespace trx {
+namespace {
+
+template <typename T, int CP, int MQ, int WAVES, int KT, bool DIST, bool CAP>
+__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 4 ? 2 : 1)))
+attention_fwd_kernel(Call call, float* part) {
+    constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
+    __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
+    const Args& a = call.a;
+    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
+    const int b = call.kv(blockIdx.x), hk = blockIdx.x - b * a.kv_heads, G = call.group.by, C = a.channels;
+    T* out = static_cast<T*>(a.out);
+    if (b == a.num_graphs) {
+        if (!part && hk == 0)
+            zero_rest(out, a.q_ptr, b, a.num_queries, (int64_t)a.heads * C, blockIdx.y * kThreads + threadIdx.x,
+                      gridDim.y * kThreads);
+        return;
+    }
+    const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
+    const int rows = qs.n * G;
+    int first = 0, last = ks.n;
+    if (gridDim.z > 1) {
+        const int each = ((ks.n + KT - 1) / KT + gridDim.z - 1) / gridDim.z * KT;
+        first = min((int64_t)ks.n, (int64_t)blockIdx.z * each);
+        last = min(ks.n, first + each);
+    }
+    const T* k_base = static_cast<const T*>(a.k) + (ks.at + first) * a.k_row + hk * a.k_head;
+    const T* v_base = static_cast<const T*>(a.v) + (ks.at + first) * a.v_row + hk * a.v_head;
+
+    for (int tile = blockIdx.y; (int64_t)tile * kRows < rows; tile += gridDim.y) {
+        const int row0 = tile * kRows + w * 16 * MQ;
+        Staged<T, CP, KT, kThreads> k_next, v_next;
+        k_next.start(k_base, a.k_row);
+        v_next.start(v_base, a.v_row);
+        k_next.load(C, last - first, KT * a.k_row);
+        v_next.load(C, last - first, KT * a.v_row);
+        frag<T> q[MQ][kSteps];
+        const float* dist[MQ];
+        Bias bias[MQ];
+        float m[MQ], l[MQ];   // the reference point in units of log 2, the sum
+        int limit[MQ];
+        f32x4 o[MQ][CP / 16];
+#pragma unroll
+        for (int t = 0; t < MQ; ++t) {
+            const int row = min(row0 + 16 * t + c, rows - 1);
+            const int i = call.group(row), h = hk * G + (row - i * G);
+            const T* p = static_cast<const T*>(a.q) + (qs.at + i) * a.q_row + h * a.q_head;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[t][s] = 32 * s + 8 * g < C ? load_frag(p + 32 * s + 8 * g) : zero_frag<T>();
+            bias[t] = bias_of<DIST, CAP>(a, DIST && a.slope ? a.slope[h] : 0.0f);
+            if (DIST) {
+                dist[t] = a.dist + b * a.dist_graph + i * a.dist_row;
+                limit[t] = i < a.dist_rows ? min(ks.n, a.dist_cols) : 0;
+            }
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < CP / 16; ++x) o[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (int j0 = first; j0 < last; j0 += KT) {
+            __syncthreads();
+            k_next.store(k_tile);
+            v_next.store(v_tile);
+            __syncthreads();
+            f32x4 d[MQ][kTiles];
+            if (DIST && row0 < rows) {
+#pragma unroll
+                for (int t = 0; t < MQ; ++t) {
+                    const bool whole = __all(j0 + KT <= limit[t]);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) d[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
+                }
+            }
+            if (j0 + KT < last) {
+                k_next.load(C, last - j0 - KT, KT * a.k_row);
+                v_next.load(C, last - j0 - KT, KT * a.v_row);
+            }
+            if (row0 >= rows) continue;
+            f32x4 s[MQ][kTiles];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+#pragma unroll
+                for (int t = 0; t < MQ; ++t) s[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < kSteps; ++x) {
+                    const frag<T> f = load_frag(k_tile + (16 * n + c) * kRow<T, CP> + 32 * x + 8 * g);
+#pragma unroll
+                    for (int t = 0; t < MQ; ++t) s[t][n] = mma(f, q[t][x], s[t][n]);
+                }
+            }
+            frag<T> p[MQ][KT / 32];
+#pragma unroll
+            for (int t = 0; t < MQ; ++t) {
+                // scores in bias.unit, and their maximum
+#define EACH_SCORE                  \
+    _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
+                if (CAP) {
+                    EACH_SCORE s[t][n][r] = a.cap * tanh_of<T>(s[t][n][r], bias[t].pre);
+                } else if (!bias[t].plain) {
+                    EACH_SCORE s[t][n][r] *= bias[t].pre;
+                }
+                if (DIST) {
+                    const float slope = bias[t].slope;
+                    if (__all(slope < 0.0f) && ordinary(d[t])) {
+                        EACH_SCORE s[t][n][r] = __builtin_fmaf(slope, d[t][n][r], s[t][n][r]);
+                    } else {
+                        EACH_SCORE s[t][n][r] =
+                            finite(d[t][n][r]) ? __builtin_fmaf(slope, d[t][n][r], s[t][n][r]) : -INFINITY;
+                    }
+                } else if (j0 + KT > last) {
+                    EACH_SCORE if (j0 + 16 * n + 4 * g + r >= last) s[t][n][r] = -INFINITY;
+                }
+                float top = -INFINITY;
+                EACH_SCORE top = fmaxf(top, s[t][n][r]);
+                top = column_max(top) * bias[t].unit;
+                // The reference point moves only when a score passes it by 2^8: nothing is lost in float32, and the
+                // accumulators are rescaled once or twice a row instead of at every new maximum.
+                const bool move = top > m[t] + 8.0f;
+                if (__any(move)) {
+                    const float f = move ? exp2_fast(m[t] - top) : 1.0f;
+                    m[t] = move ? top : m[t];
+                    l[t] *= f;
+#pragma unroll
+                    for (int x = 0; x < CP / 16; ++x) o[t][x] = o[t][x] * f;
+                }
+                const float base = m[t] == -INFINITY ? 0.0f : -m[t], unit = bias[t].unit;
+                EACH_SCORE {
+                    const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, base));
+                    l[t] += e;
+                    p[t][n / 2][4 * (n % 2) + r] = (T)e;   // rounded to the type for the product with v
+                }
+#undef EACH_SCORE
+            }
+#pragma unroll
+            for (int x = 0; x < CP / 16; ++x)
+#pragma unroll
+                for (int u = 0; u < KT / 32; ++u) {
+                    const frag<T> f = turned<T, CP>(v_tile, 32 * u, 32 * u + 16, 16 * x, lane);
+#pragma unroll
+                    for (int t = 0; t < MQ; ++t) o[t][x] = mma(f, p[t][u], o[t][x]);
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < MQ; ++t) {
+            const float sum = column_sum(l[t]);
+            const int row = row0 + 16 * t + c;
+            if (row >= rows) continue;
+            const int i = call.group(row), h = hk * G + (row - i * G);
+            const int64_t at = (qs.at + i) * a.heads + h;
+            if (part) {   // this split's sum and accumulator, for attention_join_kernel
+                const int64_t all = a.num_queries * a.heads, mine = blockIdx.z * all + at;
+                float* stat = part + (int64_t)gridDim.z * all * C;
+                if (g == 0) {
+                    stat[2 * mine] = m[t];
+                    stat[2 * mine + 1] = sum;
+                }
+#pragma unroll
+                for (int x = 0; x < CP / 16; ++x)
+                    if (16 * x + 4 * g < C) *reinterpret_cast<f32x4*>(part + mine * C + 16 * x + 4 * g) = o[t][x];
+            } else {
+                const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (a.lse && g == 0) a.lse[at] = sum == 0.0f ? -INFINITY : m[t] + log2f(sum);
+#pragma unroll
+                for (int x = 0; x < CP / 16; ++x)
+                    if (16 * x + 4 * g < C) put4(out, static_cast<T*>(a.out_low), at * C + 16 * x + 4 * g, o[t][x] * f);
+            }
+        }
+    }
+}
+
+// out, out_low and lse from the splits' sums, rows of no graph zero: a workgroup to a (row, head), its four waves
+// each over every fourth split, two channels a lane
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_kernel(Args a, const float* part, int splits) {
+    __shared__ float sums[4][2 * kWave];
+    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, C = a.channels;
+    const int64_t all = a.num_queries * a.heads, at = blockIdx.x;
+    const Span qs = all_rows(a.q_ptr, a.num_graphs, a.num_queries);
+    const int64_t row = at / a.heads;
+    if (row < qs.at || row >= qs.at + qs.n) {
+        if (threadIdx.x < C) static_cast<T*>(a.out)[at * C + threadIdx.x] = (T)0.0f;
+        return;
+    }
+    const float* stat = part + splits * all * C;
+    const bool has = lane < splits;   // at most 64
+    const float m = has ? stat[2 * (lane * all + at)] : -INFINITY, l = has ? stat[2 * (lane * all + at) + 1] : 0.0f;
+    float top = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    // a split without a finite score adds its sum as it is: zero, or the NaN that it saw
+    const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+    float sum = m == -INFINITY ? l : l * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    float x = 0.0f, y = 0.0f;
+    const int mine = min(2 * lane, C - 2);   // every lane takes part: the factors come from lanes of all splits
+    for (int s = w; s < splits; s += 4) {
+        const float2 v = *reinterpret_cast<const float2*>(part + (s * all + at) * C + mine);
+        const float fs = __shfl(f, s);
+        x = __builtin_fmaf(v.x, fs, x);
+        y = __builtin_fmaf(v.y, fs, y);
+    }
+    sums[w][2 * lane] = x;
+    sums[w][2 * lane + 1] = y;
+    __syncthreads();
+    if (threadIdx.x < C) {
+        const int ch = threadIdx.x;
+        const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float v = ((sums[0][ch] + sums[1][ch]) + (sums[2][ch] + sums[3][ch])) * r;
+        const T t = (T)v;
+        static_cast<T*>(a.out)[at * C + ch] = t;
+        if (a.out_low) static_cast<T*>(a.out_low)[at * C + ch] = (T)(v - (float)t);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.0f ? -INFINITY : top + log2f(sum);
+}
+
+template <typename T, int CP, bool DIST, bool CAP>
+void launch_fwd(const Args& a, hipStream_t stream) {
+    const AttentionCut c = cut_fwd(a);
+    float* part = c.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
+    const Call call = call_of(a);
+    const dim3 grid((unsigned)((a.num_graphs + 1) * (int64_t)a.kv_heads), (unsigned)c.tiles, c.splits);
+    constexpr int kWide = sizeof(T) == 2 && CP <= 64 ? 64 : 32;
+    if (!c.narrow)
+        hipLaunchKernelGGL((attention_fwd_kernel<T, CP, kTilesOfWave<T, CP>, 4, kWide, DIST, CAP>), grid, dim3(256), 0,
+                           stream, call, part);
+    else if (c.mq == 2)
+        hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 2, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, part);
+    else
+        hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 1, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, part);
+    if (part)
+        hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)(a.num_queries * a.heads)), dim3(256), 0, stream, a,
+                           part, c.splits);
+}
+
+}  // namespace
+
+template <typename T>
+hipError_t launch_attention_fwd(const trx_node_attention_args& a, hipStream_t stream) {
+    return by_shape<T>(a, [&](auto cp, auto dist, auto cap) {
+        launch_fwd<T, decltype(cp)::value, decltype(dist)::value, decltype(cap)::value>(a, stream);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace trx

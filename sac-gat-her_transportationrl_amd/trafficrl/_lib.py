@@ -261,8 +261,8 @@ class TrxNodeAttentionArgs(ctypes.Structure):
         ("max_queries", _i64), ("max_nodes", _i64), ("num_queries", _i64), ("num_nodes", _i64),
         ("q", _vp), ("k", _vp), ("v", _vp), ("q_row", _i64), ("q_head", _i64), ("k_row", _i64), ("k_head", _i64),
         ("v_row", _i64), ("v_head", _i64), ("q_ptr", _vp), ("k_ptr", _vp),
-        ("dist", _vp), ("dist_graph", _i64), ("dist_row", _i64), ("slope", _vp), ("out", _vp), ("lse", _vp),
-        ("grad_out", _vp), ("grad_q", _vp), ("grad_k", _vp), ("grad_v", _vp), ("grad_slope", _vp),
+        ("dist", _vp), ("dist_graph", _i64), ("dist_row", _i64), ("slope", _vp), ("out", _vp), ("out_low", _vp),
+        ("lse", _vp), ("grad_out", _vp), ("grad_q", _vp), ("grad_k", _vp), ("grad_v", _vp), ("grad_slope", _vp),
         ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 

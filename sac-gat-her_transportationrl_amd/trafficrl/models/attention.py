@@ -42,21 +42,23 @@ def _forward(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_node
     L = _lib.load()
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if save else None
+    low = torch.empty_like(out) if save and code else None
     a = _args(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code)
     a.out, a.lse = out.data_ptr(), 0 if lse is None else lse.data_ptr()
+    a.out_low = 0 if low is None else low.data_ptr()
     need = L.trx_node_attention_workspace_bytes(a, 0)
     ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
     a.workspace, a.workspace_bytes = 0 if ws is None else ws.data_ptr(), need
     _lib.check(L.trx_node_attention_forward(a, _lib.stream_ptr(q.device)), "trx_node_attention_forward")
-    return out, lse
+    return out, lse, low
 
 
 class _NodeAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slope, ptr, k_ptr, dist, scale, cap, max_queries, max_nodes, code):
         with torch.cuda.device(q.device):
-            out, lse = _forward(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code, True)
-        ctx.save_for_backward(q, k, v, slope, ptr, k_ptr, dist, out, lse)
+            out, lse, low = _forward(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code, True)
+        ctx.save_for_backward(q, k, v, slope, ptr, k_ptr, dist, out, lse, low)
         ctx.rest = scale, cap, max_queries, max_nodes, code
         return out
 
@@ -64,7 +66,7 @@ class _NodeAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         L = _lib.load()
-        q, k, v, slope, ptr, k_ptr, dist, out, lse = ctx.saved_tensors
+        q, k, v, slope, ptr, k_ptr, dist, out, lse, low = ctx.saved_tensors
         with torch.cuda.device(q.device):
             grad_out = grad_out.contiguous()
             if grad_out.data_ptr() % 16:
@@ -73,6 +75,7 @@ class _NodeAttention(torch.autograd.Function):
             gs = torch.empty_like(slope) if slope is not None and ctx.needs_input_grad[3] else None
             a = _args(q, k, v, ptr, k_ptr, dist, slope, *ctx.rest)
             a.out, a.lse, a.grad_out = out.data_ptr(), lse.data_ptr(), grad_out.data_ptr()
+            a.out_low = 0 if low is None else low.data_ptr()
             a.grad_q, a.grad_k, a.grad_v = gq.data_ptr(), gk.data_ptr(), gv.data_ptr()
             a.grad_slope = 0 if gs is None else gs.data_ptr()
             need = L.trx_node_attention_workspace_bytes(a, 1)
