@@ -150,12 +150,21 @@ inline Divide divide_by(int d) {
     return {(uint32_t)((uint64_t(1) << (31 + s)) / d + 1), 31 + s, (uint32_t)d};
 }
 
-// the arguments of a launch
+// The arguments of a launch.  grid.x: every (tile, graph, key/value head) in this order, so that the tiles of one
+// (graph, head), which read the same keys, lie 8 k blocks apart where there are 8 k heads: on one die, behind one
+// L2.  Then kRestBlocks workgroups for the rows of no graph; they must not lie between the others, or every second
+// compute unit gets nothing else.  grid.z: the splits.
+constexpr int kRestBlocks = 16;
 struct Call {
     Args a;
-    Divide group, kv;   // by heads of a group, by key/value heads
+    Divide group, kv, units;   // by heads of a group, key/value heads, (graph, key/value head)s
+    int tiles, blocks;
 };
-inline Call call_of(const Args& a) { return {a, divide_by(a.heads / a.kv_heads), divide_by(a.kv_heads)}; }
+inline Call call_of(const Args& a, int64_t tiles) {
+    const int units = a.num_graphs * a.kv_heads;
+    return {a, divide_by(a.heads / a.kv_heads), divide_by(a.kv_heads), divide_by(units > 0 ? units : 1), (int)tiles,
+            (int)tiles * units};
+}
 
 // four elements of a result; where `low` is given, what rounding took from them goes there
 template <typename T>
@@ -211,9 +220,10 @@ __device__ __forceinline__ Span all_rows(const int64_t* ptr, int graphs, int64_t
 }
 // zeros in the rows of no graph (before the first and behind the last)
 template <typename T>
-__device__ __forceinline__ void zero_rest(T* out, const int64_t* ptr, int graphs, int64_t rows, int64_t width, int at,
-                                          int step) {
+__device__ __forceinline__ void zero_rest(T* out, const int64_t* ptr, int graphs, int64_t rows, int64_t width,
+                                          int block) {
     const Span s = all_rows(ptr, graphs, rows);
+    const int64_t at = (int64_t)block * blockDim.x + threadIdx.x, step = (int64_t)kRestBlocks * blockDim.x;
     for (int64_t e = at; e < s.at * width; e += step) out[e] = (T)0.0f;
     for (int64_t e = (s.at + s.n) * width + at; e < rows * width; e += step) out[e] = (T)0.0f;
 }

@@ -15,16 +15,18 @@ namespace {
 // (a piece costs its accumulator's round trip), up to 64 and 256 MB.
 AttentionCut cut(int64_t kept, int64_t run, int64_t units, int64_t row_bytes, int wide, int least) {
     AttentionCut c;
+    units = std::max<int64_t>(1, units);
     c.narrow = kept <= 32;
     c.mq = c.narrow && kept <= 16 ? 1 : 2;
     const int64_t each = c.narrow ? 16 * c.mq : wide;
-    c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, 65535));
-    const int64_t blocks = std::max<int64_t>(1, units * c.tiles), want = c.narrow ? 2048 : 512;
+    c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, (1 << 23) / units));   // grid.x x 256 < 2^32
+    const int64_t blocks = units * c.tiles, want = c.narrow ? 2048 : 512;
     const int64_t most = std::min<int64_t>(64, std::min(run / least, (int64_t(1) << 28) / std::max<int64_t>(1, row_bytes)));
     c.splits = (int)std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, most));
     return c;
 }
 int wide_rows(const Args& a) { return a.dtype == 0 && a.channels > 64 ? 64 : 128; }
+int wide_keys(const Args& a) { return a.channels > 64 ? 64 : 128; }
 
 }  // namespace
 
@@ -41,7 +43,7 @@ AttentionCut cut_bwd_q(const trx_node_attention_args& a) {
 AttentionCut cut_bwd_kv(const trx_node_attention_args& a) {
     const int64_t G = a.heads / a.kv_heads;
     return cut(std::min(a.max_nodes, a.num_nodes), std::min(a.max_queries, a.num_queries) * G,
-               (int64_t)a.num_graphs * a.kv_heads, a.num_nodes * a.kv_heads * a.channels * 8, wide_rows(a), 256);
+               (int64_t)a.num_graphs * a.kv_heads, a.num_nodes * a.kv_heads * a.channels * 8, wide_keys(a), 256);
 }
 
 // each row's <go, out> and slope gradient, the slope chunks' sums; the splits of one pass after the other follow

@@ -28,14 +28,14 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
-    const int b = call.kv(blockIdx.x), hk = blockIdx.x - b * a.kv_heads, G = call.group.by, C = a.channels;
+    const int G = call.group.by, C = a.channels;
     T* grad_q = static_cast<T*>(a.grad_q);
-    if (b == a.num_graphs) {
-        if (hk != 0) return;
-        const int at = blockIdx.y * kThreads + threadIdx.x, step = gridDim.y * kThreads;
-        if (!part) zero_rest(grad_q, a.q_ptr, b, a.num_queries, (int64_t)a.heads * C, at, step);
+    if ((int)blockIdx.x >= call.blocks) {
+        if (!part) zero_rest(grad_q, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
         return;
     }
+    const int tile0 = call.units(blockIdx.x), of = blockIdx.x - tile0 * call.units.by;
+    const int b = call.kv(of), hk = of - b * a.kv_heads;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
     int first = 0, last = ks.n;
@@ -47,7 +47,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     const T* k_base = static_cast<const T*>(a.k) + (ks.at + first) * a.k_row + hk * a.k_head;
     const T* v_base = static_cast<const T*>(a.v) + (ks.at + first) * a.v_row + hk * a.v_head;
 
-    for (int tile = blockIdx.y; (int64_t)tile * kRows < rows; tile += gridDim.y) {
+    for (int tile = tile0; (int64_t)tile * kRows < rows; tile += call.tiles) {
         const int row0 = tile * kRows + w * 16 * MQ;
         Staged<T, CP, KT, kThreads> k_next, v_next;
         k_next.start(k_base, a.k_row);
@@ -216,15 +216,16 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
     __shared__ __attribute__((aligned(16))) int64_t row_dist[RT];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
-    const int b = call.kv(blockIdx.x), hk = blockIdx.x - b * a.kv_heads, G = call.group.by, C = a.channels;
+    const int G = call.group.by, C = a.channels;
     T *grad_k = static_cast<T*>(a.grad_k), *grad_v = static_cast<T*>(a.grad_v);
-    if (b == a.num_graphs) {
-        if (hk != 0 || part) return;
-        const int at = blockIdx.y * kThreads + threadIdx.x, step = gridDim.y * kThreads;
-        zero_rest(grad_k, a.k_ptr, b, a.num_nodes, (int64_t)a.kv_heads * C, at, step);
-        zero_rest(grad_v, a.k_ptr, b, a.num_nodes, (int64_t)a.kv_heads * C, at, step);
+    if ((int)blockIdx.x >= call.blocks) {
+        if (part) return;
+        zero_rest(grad_k, a.k_ptr, a.num_graphs, a.num_nodes, (int64_t)a.kv_heads * C, blockIdx.x - call.blocks);
+        zero_rest(grad_v, a.k_ptr, a.num_graphs, a.num_nodes, (int64_t)a.kv_heads * C, blockIdx.x - call.blocks);
         return;
     }
+    const int tile0 = call.units(blockIdx.x), of = blockIdx.x - tile0 * call.units.by;
+    const int b = call.kv(of), hk = of - b * a.kv_heads;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
     int first = 0, last = rows;
@@ -237,7 +238,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
     const float pre = CAP ? a.scale / a.cap : plain ? 1.0f : a.scale, unit = plain ? a.scale * kLog2e : kLog2e;
     const float per = plain ? -1.0f / a.scale : -1.0f;
 
-    for (int tile = blockIdx.y; (int64_t)tile * kKeys < ks.n; tile += gridDim.y) {
+    for (int tile = tile0; (int64_t)tile * kKeys < ks.n; tile += call.tiles) {
         const int key0 = tile * kKeys + w * 16 * MK;
         frag<T> k[MK][kSteps], v[MK][kSteps];
         const float* dist[MK];
@@ -465,14 +466,13 @@ void launch_bwd(const Args& a, hipStream_t stream) {
     float *dots = static_cast<float*>(a.workspace), *slopes = dots + a.num_queries * a.heads;
     float *chunks = slopes + a.num_queries * a.heads, *split = dots + attention_row_floats(a);
     const bool want_slopes = DIST && a.grad_slope && a.slope;
-    const Call call = call_of(a);
-    const unsigned gx = (unsigned)((a.num_graphs + 1) * (int64_t)a.kv_heads);
     auto blocks = [](int64_t n) { return (unsigned)std::min<int64_t>(2048, (n / 4 + 255) / 256); };
-    constexpr int M = kTilesOfWave<T, CP>;
+    constexpr int M = kTilesOfWave<T, CP>, MK = CP == 128 ? 1 : 2;
     if (a.num_queries > 0) {
         const AttentionCut c = cut_bwd_q(a);
         float* part = c.splits > 1 ? split : nullptr;
-        const dim3 grid(gx, (unsigned)c.tiles, c.splits);
+        const Call call = call_of(a, c.tiles);
+        const dim3 grid(call.blocks + kRestBlocks, 1, c.splits);
         if (c.narrow)
             hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, M, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
                                want_slopes ? slopes : nullptr, part);
@@ -498,12 +498,13 @@ void launch_bwd(const Args& a, hipStream_t stream) {
     if (a.num_nodes > 0) {
         const AttentionCut c = cut_bwd_kv(a);
         float* part = c.splits > 1 ? split : nullptr;
-        const dim3 grid(gx, (unsigned)c.tiles, c.splits);
+        const Call call = call_of(a, c.tiles);
+        const dim3 grid(call.blocks + kRestBlocks, 1, c.splits);
         if (c.narrow)
-            hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, M, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
+            hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, MK, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
                                part);
         else
-            hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, M, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call,
+            hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, MK, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call,
                                dots, part);
         if (part) {
             const int64_t n = a.num_nodes * a.kv_heads * a.channels;

@@ -21,14 +21,14 @@ attention_fwd_kernel(Call call, float* part) {
     __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
-    const int b = call.kv(blockIdx.x), hk = blockIdx.x - b * a.kv_heads, G = call.group.by, C = a.channels;
+    const int G = call.group.by, C = a.channels;
     T* out = static_cast<T*>(a.out);
-    if (b == a.num_graphs) {
-        if (!part && hk == 0)
-            zero_rest(out, a.q_ptr, b, a.num_queries, (int64_t)a.heads * C, blockIdx.y * kThreads + threadIdx.x,
-                      gridDim.y * kThreads);
+    if ((int)blockIdx.x >= call.blocks) {
+        if (!part) zero_rest(out, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
         return;
     }
+    const int tile0 = call.units(blockIdx.x), unit = blockIdx.x - tile0 * call.units.by;
+    const int b = call.kv(unit), hk = unit - b * a.kv_heads;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
     int first = 0, last = ks.n;
@@ -40,7 +40,7 @@ attention_fwd_kernel(Call call, float* part) {
     const T* k_base = static_cast<const T*>(a.k) + (ks.at + first) * a.k_row + hk * a.k_head;
     const T* v_base = static_cast<const T*>(a.v) + (ks.at + first) * a.v_row + hk * a.v_head;
 
-    for (int tile = blockIdx.y; (int64_t)tile * kRows < rows; tile += gridDim.y) {
+    for (int tile = tile0; (int64_t)tile * kRows < rows; tile += call.tiles) {
         const int row0 = tile * kRows + w * 16 * MQ;
         Staged<T, CP, KT, kThreads> k_next, v_next;
         k_next.start(k_base, a.k_row);
@@ -181,7 +181,35 @@ attention_fwd_kernel(Call call, float* part) {
     }
 }
 
-// out, out_low and lse from the splits' sums, rows of no graph zero: a workgroup to a (row, head), its four waves
+// out, out_low and lse from few splits' sums, rows of no graph zero: four channels a thread
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_few_kernel(Args a, const float* part, int splits) {
+    const Span qs = all_rows(a.q_ptr, a.num_graphs, a.num_queries);
+    const int C = a.channels, C4 = C / 4;
+    const int64_t all = a.num_queries * a.heads, step = (int64_t)gridDim.x * 256;
+    const float* stat = part + splits * all * C;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all * C4; x += step) {
+        const int64_t at = x / C4, row = at / a.heads, e = x * 4;
+        if (row < qs.at || row >= qs.at + qs.n) {
+            put4(static_cast<T*>(a.out), static_cast<T*>(nullptr), e, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+            continue;
+        }
+        float top = -INFINITY, sum = 0.0f;
+        for (int s = 0; s < splits; ++s) top = fmaxf(top, stat[2 * (s * all + at)]);
+        f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < splits; ++s) {
+            const float m = stat[2 * (s * all + at)], l = stat[2 * (s * all + at) + 1];
+            // a split without a finite score adds its sum as it is: zero, or the NaN that it saw
+            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+            sum += m == -INFINITY ? l : l * f;
+            v = v + *reinterpret_cast<const f32x4*>(part + s * all * C + e) * f;
+        }
+        put4(static_cast<T*>(a.out), static_cast<T*>(a.out_low), e, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
+        if (a.lse && x == at * C4) a.lse[at] = sum == 0.0f ? -INFINITY : top + log2f(sum);
+    }
+}
+
+// The same from many: a workgroup to a (row, head), its four waves
 // each over every fourth split, two channels a lane
 template <typename T>
 __global__ void __launch_bounds__(256) attention_join_kernel(Args a, const float* part, int splits) {
@@ -231,8 +259,8 @@ template <typename T, int CP, bool DIST, bool CAP>
 void launch_fwd(const Args& a, hipStream_t stream) {
     const AttentionCut c = cut_fwd(a);
     float* part = c.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
-    const Call call = call_of(a);
-    const dim3 grid((unsigned)((a.num_graphs + 1) * (int64_t)a.kv_heads), (unsigned)c.tiles, c.splits);
+    const Call call = call_of(a, c.tiles);
+    const dim3 grid(call.blocks + kRestBlocks, 1, c.splits);
     constexpr int kWide = sizeof(T) == 2 && CP <= 64 ? 64 : 32;
     if (!c.narrow)
         hipLaunchKernelGGL((attention_fwd_kernel<T, CP, kTilesOfWave<T, CP>, 4, kWide, DIST, CAP>), grid, dim3(256), 0,
@@ -241,7 +269,11 @@ void launch_fwd(const Args& a, hipStream_t stream) {
         hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 2, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, part);
     else
         hipLaunchKernelGGL((attention_fwd_kernel<T, CP, 1, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, part);
-    if (part)
+    if (part && c.splits <= 8)
+        hipLaunchKernelGGL(attention_join_few_kernel<T>,
+                           dim3((unsigned)std::min<int64_t>(4096, (a.num_queries * a.heads * a.channels / 4 + 255) / 256)),
+                           dim3(256), 0, stream, a, part, c.splits);
+    else if (part)
         hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)(a.num_queries * a.heads)), dim3(256), 0, stream, a,
                            part, c.splits);
 }
