@@ -100,37 +100,28 @@ __device__ __forceinline__ frag<T> turned(const T* tile, int row0, int row1, int
 }
 
 // ROWS x CP elements of consecutive rows on their way from memory to LDS through
-// registers: loaded while the tile before is worked on
+// registers.  Rows and channels behind the last come from the last: nothing is
+// masked, because what a tile holds there meets weights of zero (rows) or zero
+// operands and results that are not stored (channels).
 template <typename T, int CP, int ROWS, int THREADS>
 struct Staged {
     static constexpr int kChunks = ROWS * (CP / 8), kEach = (kChunks + THREADS - 1) / THREADS;
     Eight<T> r[kEach];
-    const T* p[kEach];
 
     static __device__ __forceinline__ int row_of(int e) { return (threadIdx.x + e * THREADS) / (CP / 8); }
     static __device__ __forceinline__ int channel_of(int e) { return 8 * ((threadIdx.x + e * THREADS) % (CP / 8)); }
 
-    __device__ __forceinline__ void start(const T* first, int64_t row) {
+    // rows first .. of `rows` (at least one)
+    __device__ __forceinline__ void load(const T* base, int64_t row, int first, int rows, int C) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) p[e] = first + row_of(e) * row + channel_of(e);
-    }
-    // `left` rows are there; step: ROWS rows on
-    __device__ __forceinline__ void load(int C, int left, int64_t step) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const bool in = row_of(e) < left && row_of(e) < ROWS && channel_of(e) < C;
-            r[e] = in ? load8(p[e]) : Eight<T>{};
-            p[e] += step;
-        }
+        for (int e = 0; e < kEach; ++e)
+            r[e] = load8(base + min(first + row_of(e), rows - 1) * row + min(channel_of(e), C - 8));
     }
     // the same with a pointer of its own for each row
     template <typename F>
-    __device__ __forceinline__ void load_rows(int C, int left, F&& row) {
+    __device__ __forceinline__ void load_rows(int first, int rows, int C, F&& row) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const bool in = row_of(e) < left && row_of(e) < ROWS && channel_of(e) < C;
-            r[e] = in ? load8(row(row_of(e)) + channel_of(e)) : Eight<T>{};
-        }
+        for (int e = 0; e < kEach; ++e) r[e] = load8(row(min(first + row_of(e), rows - 1)) + min(channel_of(e), C - 8));
     }
     __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
@@ -154,6 +145,8 @@ inline Divide divide_by(int d) {
 // (graph, head), which read the same keys, lie 8 k blocks apart where there are 8 k heads: on one die, behind one
 // L2.  Then kRestBlocks workgroups for the rows of no graph; they must not lie between the others, or every second
 // compute unit gets nothing else.  grid.z: the splits.
+// Where there are distances, each die gets consecutive (tile, graph, head)s instead: the heads of a tile read the
+// same distances, 4 bytes a pair and head that would otherwise come through the fabric once a die.
 constexpr int kRestBlocks = 16;
 struct Call {
     Args a;
@@ -187,6 +180,10 @@ __device__ __forceinline__ void put4(T* out, T* low, int64_t at, f32x4 v) {
 template <typename T, int CP>
 constexpr int kTilesOfWave = sizeof(T) == 4 && CP == 128 ? 1 : 2;
 
+// waves of a SIMD that registers are left for
+template <typename T, int CP, int WAVES>
+constexpr int kWavesPerSimd = WAVES > 1 ? 2 : 1;
+
 // calls f with the padded channels, whether there are distances, whether scores are capped
 template <typename T, typename F>
 inline hipError_t by_shape(const Args& a, F&& f) {
@@ -198,6 +195,12 @@ inline hipError_t by_shape(const Args& a, F&& f) {
     if (a.channels <= 32) return second(std::integral_constant<int, 32>{});
     if (a.channels <= 64) return second(std::integral_constant<int, 64>{});
     return second(std::integral_constant<int, 128>{});
+}
+
+template <bool DIST>
+__device__ __forceinline__ int work_of(const Call& call) {
+    const int id = blockIdx.x, each = call.blocks / 8;   // 8 dies take workgroups in turn
+    return DIST && id < 8 * each ? id % 8 * each + id / 8 : id;
 }
 
 struct Span {
@@ -286,10 +289,13 @@ __device__ __forceinline__ bool ordinary(const f32x4 (&d)[N]) {
 
 // one column's four distances behind key j: +inf from `limit` on
 __device__ __forceinline__ f32x4 distances(const float* row, int j, int limit, bool whole) {
-    if (whole) return *reinterpret_cast<const f32x4u*>(row + j);
-    f32x4 d;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) d[r] = j + r < limit ? row[j + r] : INFINITY;
+    if (whole || j + 4 <= limit) return *reinterpret_cast<const f32x4u*>(row + j);
+    f32x4 d{INFINITY, INFINITY, INFINITY, INFINITY};
+    if (j < limit) {
+        d[0] = row[j];
+        if (j + 1 < limit) d[1] = row[j + 1];
+        if (j + 2 < limit) d[2] = row[j + 2];
+    }
     return d;
 }
 

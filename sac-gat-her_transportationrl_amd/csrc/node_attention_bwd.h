@@ -22,9 +22,10 @@ struct SlopeSums {
 };
 
 template <typename T, int CP, int MQ, int WAVES, int KT, bool DIST, bool CAP>
-__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 4 ? 2 : 1)))
+__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, CP, WAVES>)))
 attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
+    constexpr bool kAhead = WAVES > 1;   // one wave's registers are better spent on more waves
     __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
@@ -34,7 +35,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
         if (!part) zero_rest(grad_q, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
         return;
     }
-    const int tile0 = call.units(blockIdx.x), of = blockIdx.x - tile0 * call.units.by;
+    const int tile0 = call.units(work_of<DIST>(call)), of = work_of<DIST>(call) - tile0 * call.units.by;
     const int b = call.kv(of), hk = of - b * a.kv_heads;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
@@ -44,16 +45,17 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
         first = min((int64_t)ks.n, (int64_t)blockIdx.z * each);
         last = min(ks.n, first + each);
     }
-    const T* k_base = static_cast<const T*>(a.k) + (ks.at + first) * a.k_row + hk * a.k_head;
-    const T* v_base = static_cast<const T*>(a.v) + (ks.at + first) * a.v_row + hk * a.v_head;
+    const T* k_base = static_cast<const T*>(a.k) + ks.at * a.k_row + hk * a.k_head;
+    const T* v_base = static_cast<const T*>(a.v) + ks.at * a.v_row + hk * a.v_head;
 
     for (int tile = tile0; (int64_t)tile * kRows < rows; tile += call.tiles) {
         const int row0 = tile * kRows + w * 16 * MQ;
         Staged<T, CP, KT, kThreads> k_next, v_next;
-        k_next.start(k_base, a.k_row);
-        v_next.start(v_base, a.v_row);
-        k_next.load(C, last - first, KT * a.k_row);
-        v_next.load(C, last - first, KT * a.v_row);
+        auto fetch = [&](int j0) {
+            k_next.load(k_base, a.k_row, j0, ks.n, C);
+            v_next.load(v_base, a.v_row, j0, ks.n, C);
+        };
+        if (kAhead && first < last) fetch(first);
         frag<T> q[MQ][kSteps], go[MQ][kSteps];
         const float* dist[MQ];
         Bias bias[MQ];
@@ -97,12 +99,9 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) acc[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        f32x4 d[MQ][kTiles];
         for (int j0 = first; j0 < last; j0 += KT) {
-            __syncthreads();
-            k_next.store(k_tile);
-            v_next.store(v_tile);
-            __syncthreads();
-            f32x4 d[MQ][kTiles];
+            if (!kAhead) fetch(j0);
             if (DIST && row0 < rows) {
 #pragma unroll
                 for (int t = 0; t < MQ; ++t) {
@@ -111,10 +110,11 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
                     for (int n = 0; n < kTiles; ++n) d[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
                 }
             }
-            if (j0 + KT < last) {
-                k_next.load(C, last - j0 - KT, KT * a.k_row);
-                v_next.load(C, last - j0 - KT, KT * a.v_row);
-            }
+            __syncthreads();
+            k_next.store(k_tile);
+            v_next.store(v_tile);
+            __syncthreads();
+            if (kAhead && j0 + KT < last) fetch(j0 + KT);
             if (row0 >= rows) continue;
             f32x4 s[MQ][kTiles], gp[MQ][kTiles];
 #pragma unroll
@@ -208,12 +208,12 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
 }
 
 template <typename T, int CP, int MK, int WAVES, int RT, bool DIST, bool CAP>
-__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 4 ? 2 : 1)))
+__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, CP, WAVES>)))
 attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
     constexpr int kThreads = kWave * WAVES, kKeys = 16 * MK * WAVES, kSteps = CP / 32, kTiles = RT / 16;
+    constexpr bool kAhead = WAVES > 1;
     __shared__ __attribute__((aligned(16))) T q_tile[RT * kRow<T, CP>], go_tile[RT * kRow<T, CP>];
     __shared__ __attribute__((aligned(16))) float row_lse[RT], row_D[RT], row_slope[RT];
-    __shared__ __attribute__((aligned(16))) int64_t row_dist[RT];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
     const int G = call.group.by, C = a.channels;
@@ -224,7 +224,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         zero_rest(grad_v, a.k_ptr, a.num_graphs, a.num_nodes, (int64_t)a.kv_heads * C, blockIdx.x - call.blocks);
         return;
     }
-    const int tile0 = call.units(blockIdx.x), of = blockIdx.x - tile0 * call.units.by;
+    const int tile0 = call.units(work_of<DIST>(call)), of = work_of<DIST>(call) - tile0 * call.units.by;
     const int b = call.kv(of), hk = of - b * a.kv_heads;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
@@ -237,6 +237,10 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
     const bool plain = !CAP && a.scale > 1e-18f;
     const float pre = CAP ? a.scale / a.cap : plain ? 1.0f : a.scale, unit = plain ? a.scale * kLog2e : kLog2e;
     const float per = plain ? -1.0f / a.scale : -1.0f;
+    bool falls = DIST && a.slope;   // all the group's slopes are positive
+    if (falls)
+        for (int h = lane; h < G; h += kWave) falls = falls && a.slope[hk * G + h] > 0.0f && a.slope[hk * G + h] < 1e18f;
+    falls = __all(falls);
 
     for (int tile = tile0; (int64_t)tile * kKeys < ks.n; tile += call.tiles) {
         const int key0 = tile * kKeys + w * 16 * MK;
@@ -260,60 +264,59 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         }
         Staged<T, CP, RT, kThreads> q_next, go_next;
         float next_lse = 0.0f, next_D = 0.0f, next_slope = 0.0f;
-        int64_t next_dist = -1;
         auto fetch = [&](int r0) {
-            const int left = last - r0;
-            q_next.load_rows(C, left, [&](int x) {
-                const int i = call.group(r0 + x), h = hk * G + (r0 + x - i * G);
+            q_next.load_rows(r0, rows, C, [&](int row) {
+                const int i = call.group(row), h = hk * G + (row - i * G);
                 return static_cast<const T*>(a.q) + (qs.at + i) * a.q_row + h * a.q_head;
             });
-            go_next.load_rows(C, left, [&](int x) {
-                const int i = call.group(r0 + x), h = hk * G + (r0 + x - i * G);
+            go_next.load_rows(r0, rows, C, [&](int row) {
+                const int i = call.group(row), h = hk * G + (row - i * G);
                 return static_cast<const T*>(a.grad_out) + ((qs.at + i) * a.heads + h) * C;
             });
             next_lse = INFINITY;   // rows that are not there, and empty ones: every probability comes out as zero
-            next_D = next_slope = 0.0f;
-            next_dist = -1;
-            if (threadIdx.x < RT && (int)threadIdx.x < left) {
+            next_D = 0.0f;
+            next_slope = -1.0f;    // as any row's where all fall: with 0, a distance of +inf would make NaN
+            if (threadIdx.x < RT && r0 + (int)threadIdx.x < last) {
                 const int row = r0 + threadIdx.x, i = call.group(row), h = hk * G + (row - i * G);
                 const int64_t at = (qs.at + i) * a.heads + h;
                 if (a.lse[at] != -INFINITY) {
                     next_lse = a.lse[at];
                     next_D = dots[at];
                 }
-                if (DIST) {
-                    next_slope = a.slope ? a.slope[h] * per : 0.0f;
-                    if (i < a.dist_rows) next_dist = i * a.dist_row;
-                }
+                if (DIST) next_slope = a.slope ? a.slope[h] * per : 0.0f;
             }
         };
-        if (first < last) fetch(first);
+        f32x4 d[MK][kTiles];
+        if (kAhead && first < last) fetch(first);
         for (int r0 = first; r0 < last; r0 += RT) {
+            if (!kAhead) fetch(r0);
+            if (DIST && key0 < ks.n) {
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = min(r0 + 16 * n + 4 * g + r, rows - 1), i = call.group(row);
+                        const int64_t at = i * a.dist_row;
+                        const bool in = i < a.dist_rows;
+#pragma unroll
+                        for (int t = 0; t < MK; ++t) d[t][n][r] = in && dist[t] ? dist[t][at] : INFINITY;
+                    }
+            }
             __syncthreads();
             q_next.store(q_tile);
             go_next.store(go_tile);
             if (threadIdx.x < RT) {
                 row_lse[threadIdx.x] = next_lse;
                 row_D[threadIdx.x] = next_D;
-                if (DIST) {
-                    row_slope[threadIdx.x] = next_slope;
-                    row_dist[threadIdx.x] = next_dist;
-                }
+                if (DIST) row_slope[threadIdx.x] = next_slope;
             }
             __syncthreads();
-            if (r0 + RT < last) fetch(r0 + RT);
+            if (kAhead && r0 + RT < last) fetch(r0 + RT);
             if (key0 >= ks.n) continue;
-            f32x4 d[MK][kTiles];
-            if (DIST) {
+            bool free = falls;
+            if (DIST)
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int64_t at = row_dist[16 * n + 4 * g + r];
-#pragma unroll
-                        for (int t = 0; t < MK; ++t) d[t][n][r] = dist[t] && at >= 0 ? dist[t][at] : INFINITY;
-                    }
-            }
+                for (int t = 0; t < MK; ++t) free = free && ordinary(d[t]);
             f32x4 s[MK][kTiles], gp[MK][kTiles];
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
@@ -350,7 +353,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                         } else if (!plain) {
                             z = z * pre;
                         }
-                        if (DIST) z = finite(d[t][n][r]) ? __builtin_fmaf(slope[r], d[t][n][r], z) : -INFINITY;
+                        if (DIST) z = free || finite(d[t][n][r]) ? __builtin_fmaf(slope[r], d[t][n][r], z) : -INFINITY;
                         const float e = exp2_fast(__builtin_fmaf(z, unit, -lse[r]));
                         const float v = e * (gp[t][n][r] - D[r]), x = CAP ? v * slack : v;
                         p[t][n / 2][4 * (n % 2) + r] = (T)e;   // both rounded to the type for their products

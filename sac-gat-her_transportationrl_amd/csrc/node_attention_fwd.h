@@ -15,9 +15,11 @@ namespace trx {
 namespace {
 
 template <typename T, int CP, int MQ, int WAVES, int KT, bool DIST, bool CAP>
-__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 4 ? 2 : 1)))
+__global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, CP, WAVES>)))
 attention_fwd_kernel(Call call, float* part) {
     constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
+    constexpr bool kAhead = WAVES > 1;   // one wave's registers are better spent on more waves
+    constexpr bool kAheadD = kAhead && CP == 128;   // registers for the next tile's distances: at 64 channels they cost more than they hide
     __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
@@ -27,7 +29,7 @@ attention_fwd_kernel(Call call, float* part) {
         if (!part) zero_rest(out, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
         return;
     }
-    const int tile0 = call.units(blockIdx.x), unit = blockIdx.x - tile0 * call.units.by;
+    const int tile0 = call.units(work_of<DIST>(call)), unit = work_of<DIST>(call) - tile0 * call.units.by;
     const int b = call.kv(unit), hk = unit - b * a.kv_heads;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
@@ -37,16 +39,17 @@ attention_fwd_kernel(Call call, float* part) {
         first = min((int64_t)ks.n, (int64_t)blockIdx.z * each);
         last = min(ks.n, first + each);
     }
-    const T* k_base = static_cast<const T*>(a.k) + (ks.at + first) * a.k_row + hk * a.k_head;
-    const T* v_base = static_cast<const T*>(a.v) + (ks.at + first) * a.v_row + hk * a.v_head;
+    const T* k_base = static_cast<const T*>(a.k) + ks.at * a.k_row + hk * a.k_head;
+    const T* v_base = static_cast<const T*>(a.v) + ks.at * a.v_row + hk * a.v_head;
 
     for (int tile = tile0; (int64_t)tile * kRows < rows; tile += call.tiles) {
         const int row0 = tile * kRows + w * 16 * MQ;
         Staged<T, CP, KT, kThreads> k_next, v_next;
-        k_next.start(k_base, a.k_row);
-        v_next.start(v_base, a.v_row);
-        k_next.load(C, last - first, KT * a.k_row);
-        v_next.load(C, last - first, KT * a.v_row);
+        auto fetch = [&](int j0) {
+            k_next.load(k_base, a.k_row, j0, ks.n, C);
+            v_next.load(v_base, a.v_row, j0, ks.n, C);
+        };
+        if (kAhead && first < last) fetch(first);
         frag<T> q[MQ][kSteps];
         const float* dist[MQ];
         Bias bias[MQ];
@@ -70,23 +73,30 @@ attention_fwd_kernel(Call call, float* part) {
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) o[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        f32x4 d[MQ][kTiles], d_next[MQ][kTiles];
+        auto fetch_distances = [&](int j0, f32x4(&to)[MQ][kTiles]) {
+#pragma unroll
+            for (int t = 0; t < MQ; ++t) {
+                const bool whole = __all(j0 + KT <= limit[t]);
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) to[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
+            }
+        };
+        if (DIST && kAheadD && first < last && row0 < rows) fetch_distances(first, d_next);
         for (int j0 = first; j0 < last; j0 += KT) {
+            if (!kAhead) fetch(j0);
+            if (DIST && !kAheadD && row0 < rows) fetch_distances(j0, d);
             __syncthreads();
             k_next.store(k_tile);
             v_next.store(v_tile);
             __syncthreads();
-            f32x4 d[MQ][kTiles];
-            if (DIST && row0 < rows) {
+            if (kAhead && j0 + KT < last) fetch(j0 + KT);
+            if (DIST && kAheadD && row0 < rows) {
 #pragma unroll
-                for (int t = 0; t < MQ; ++t) {
-                    const bool whole = __all(j0 + KT <= limit[t]);
+                for (int t = 0; t < MQ; ++t)
 #pragma unroll
-                    for (int n = 0; n < kTiles; ++n) d[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
-                }
-            }
-            if (j0 + KT < last) {
-                k_next.load(C, last - j0 - KT, KT * a.k_row);
-                v_next.load(C, last - j0 - KT, KT * a.v_row);
+                    for (int n = 0; n < kTiles; ++n) d[t][n] = d_next[t][n];
+                if (j0 + KT < last) fetch_distances(j0 + KT, d_next);
             }
             if (row0 >= rows) continue;
             f32x4 s[MQ][kTiles];
