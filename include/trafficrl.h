@@ -960,7 +960,7 @@ int trx_action_log_probs_backward(const trx_action_log_probs_args* a, void* stre
  * first) of the four words of Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011)
  * with counter (e / 8 low, e / 8 high, step mod 2^32, site) and key (seed low,
  * seed high).  rng int64 [2] (device): (seed, step); the forward writes the
- * pair it used to rng_used, from which the backward, grad_x = keep * grad_y *
+ * pair it used to rng_used (NULL: not wanted), from which the backward, grad_x = keep * grad_y *
  * 65536 / (65536 - border), draws the same bits again: no mask is stored and
  * rng may move on in between.  Pointers aligned to 16 bytes.               */
 int trx_dropout_add_forward(int64_t n, int32_t dtype, const void* x, const void* residual, const int64_t* rng,

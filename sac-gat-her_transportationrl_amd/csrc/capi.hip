@@ -1394,7 +1394,7 @@ int check_log_probs(const trx_action_log_probs_args* a, bool backward) {
     if (rc) return rc;
     if (a->rows > 0) {
         if (!a->logits && (a->row_ptr ? a->total : a->row_len) > 0) return fail(TRX_EINVAL, "action_log_probs: NULL logits");
-        if (!a->action || !a->stats || !a->log_prob || !a->entropy)
+        if (!a->action || !a->stats || (!backward && (!a->log_prob || !a->entropy)))
             return fail(TRX_EINVAL, "action_log_probs: NULL action / log_prob / entropy / stats");
         if (a->top_k > 0 && !a->top_action) return fail(TRX_EINVAL, "action_log_probs: NULL top_action");
         if (!backward && a->top_k > 0 && !a->top_log_prob) return fail(TRX_EINVAL, "action_log_probs: NULL top_log_prob");
@@ -1468,8 +1468,7 @@ int trx_dropout_add_forward(int64_t n, int32_t dtype, const void* x, const void*
                             int32_t border, uint32_t site, void* y, int64_t* rng_used, void* stream) {
     int rc = check_dropout(n, dtype, x, rng, border, y);
     if (rc) return rc;
-    if (n > 0 && (!rng_used || misaligned(residual)))
-        return fail(TRX_EINVAL, "dropout_add: NULL rng_used or a residual that is not 16-byte aligned");
+    if (misaligned(residual)) return fail(TRX_EINVAL, "dropout_add: buffers must be 16-byte aligned");
     if (n == 0) return TRX_OK;
     hipError_t e = trx::launch_dropout_add(n, dtype, x, residual, rng, border, site, y, rng_used,
                                            static_cast<hipStream_t>(stream));

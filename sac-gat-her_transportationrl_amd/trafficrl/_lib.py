@@ -456,27 +456,54 @@ def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
-# dtype codes of the entry points that take all three
-FLOAT_CODES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_float_codes = {}
 
 
 def float_code(t, what: str) -> int:
-    code = FLOAT_CODES.get(str(t.dtype))
+    """The dtype code of the entry points that take all three float types."""
+    if not _float_codes:
+        import torch
+        _float_codes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    code = _float_codes.get(t.dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
 
 
-def on_device(what: str, first, *others):
-    """ValueError unless every tensor (None: skipped) lies on the first one's HIP
-    device; returns a context in which that device is the current one."""
-    import torch
+def same_device(what: str, first, *others):
+    """ValueError unless every tensor (None: skipped) lies on the first one's HIP device."""
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
-    if not first.is_cuda:
-        raise ValueError(f"{what} needs tensors on a HIP device, got {first.device} (there is no CPU fallback)")
-    return torch.cuda.device(first.device)
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+    if device.type != "cuda":
+        raise ValueError(f"{what} needs tensors on a HIP device, got {device} (there is no CPU fallback)")
+
+
+def on_device(device, f, *args):
+    """f(*args) with `device` the current one: launches go to the current device."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return f(*args)
+    with torch.cuda.device(device):
+        return f(*args)
+
+
+def raw_stream(device) -> int:
+    """The current HIP stream of a device, as the entry points' void*."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def once(backward):
+    """once_differentiable without its cost where no second derivative is asked for."""
+    import torch
+    from torch.autograd.function import once_differentiable
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def stream_ptr(device=None) -> ctypes.c_void_p:

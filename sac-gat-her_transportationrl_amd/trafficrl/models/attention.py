@@ -7,7 +7,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -23,66 +22,67 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _args(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code):
-    a = _lib.TrxNodeAttentionArgs()
-    a.num_graphs, a.heads, a.kv_heads, a.channels, a.dtype = ptr.numel() - 1, q.shape[1], k.shape[1], q.shape[2], code
-    a.scale, a.cap, a.max_queries, a.max_nodes = scale, cap, max_queries, max_nodes
-    a.num_queries, a.num_nodes = q.shape[0], k.shape[0]
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    (a.q_row, a.q_head, _), (a.k_row, a.k_head, _), (a.v_row, a.v_head, _) = q.stride(), k.stride(), v.stride()
-    a.q_ptr, a.k_ptr = ptr.data_ptr(), k_ptr.data_ptr()
+def _args(q, k, v, ptr, k_ptr, dist, slope, rest, out, low, lse, backward: bool, grads=(0, 0, 0, 0, 0)):
+    """The argument block and the workspace it points to."""
+    scale, cap, max_queries, max_nodes, code = rest
+    rows, heads, channels = q.shape
+    nodes, kv_heads, _ = k.shape
+    q_row, q_head, _ = q.stride()
+    k_row, k_head, _ = k.stride()
+    v_row, v_head, _ = v.stride()
+    d = (0, 0, 0, 0, 0, 0)
     if dist is not None:
-        a.dist_rows, a.dist_cols = dist.shape[-2:]
-        a.dist, a.dist_graph, a.dist_row = dist.data_ptr(), dist.stride(0) if dist.dim() == 3 else 0, dist.stride(-2)
-        a.slope = 0 if slope is None else slope.data_ptr()
-    return a
+        d = (*dist.shape[-2:], dist.data_ptr(), dist.stride(0) if dist.dim() == 3 else 0, dist.stride(-2),
+             0 if slope is None else slope.data_ptr())
+    a = _lib.TrxNodeAttentionArgs(
+        ptr.numel() - 1, heads, kv_heads, channels, code, d[0], d[1], scale, cap, max_queries, max_nodes, rows, nodes,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_row, q_head, k_row, k_head, v_row, v_head, ptr.data_ptr(),
+        k_ptr.data_ptr(), *d[2:], out.data_ptr(), 0 if low is None else low.data_ptr(),
+        0 if lse is None else lse.data_ptr(), *grads)
+    need = _lib.load().trx_node_attention_workspace_bytes(a, backward)
+    ws = None
+    if need > 0:
+        ws = torch.empty(need, device=q.device, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    return a, ws
 
 
-def _forward(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code, save: bool):
-    L = _lib.load()
+def _launch(q, k, v, ptr, k_ptr, dist, slope, rest, save: bool):
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if save else None
-    low = torch.empty_like(out) if save and code else None
-    a = _args(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code)
-    a.out, a.lse = out.data_ptr(), 0 if lse is None else lse.data_ptr()
-    a.out_low = 0 if low is None else low.data_ptr()
-    need = L.trx_node_attention_workspace_bytes(a, 0)
-    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
-    a.workspace, a.workspace_bytes = 0 if ws is None else ws.data_ptr(), need
-    _lib.check(L.trx_node_attention_forward(a, _lib.stream_ptr(q.device)), "trx_node_attention_forward")
-    return out, lse, low
+    lse = low = None
+    if save:
+        lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32)
+        low = torch.empty_like(out) if out.dtype != torch.float32 else None
+    a, ws = _args(q, k, v, ptr, k_ptr, dist, slope, rest, out, low, lse, False)
+    _lib.check(_lib.load().trx_node_attention_forward(a, _lib.raw_stream(q.device)), "trx_node_attention_forward")
+    return out, low, lse
+
+
+def _launch_backward(q, k, v, slope, ptr, k_ptr, dist, out, low, lse, rest, grad_out, wants_slope):
+    grad_out = grad_out.contiguous()
+    if grad_out.data_ptr() % 16:
+        grad_out = grad_out.clone()
+    gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+    gs = torch.empty_like(slope) if wants_slope else None
+    a, ws = _args(q, k, v, ptr, k_ptr, dist, slope, rest, out, low, lse, True,
+                  (grad_out.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), 0 if gs is None else gs.data_ptr()))
+    _lib.check(_lib.load().trx_node_attention_backward(a, _lib.raw_stream(q.device)), "trx_node_attention_backward")
+    return gq, gk, gv, gs
 
 
 class _NodeAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, slope, ptr, k_ptr, dist, scale, cap, max_queries, max_nodes, code):
-        with torch.cuda.device(q.device):
-            out, lse, low = _forward(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code, True)
-        ctx.save_for_backward(q, k, v, slope, ptr, k_ptr, dist, out, lse, low)
-        ctx.rest = scale, cap, max_queries, max_nodes, code
+    def forward(ctx, q, k, v, slope, ptr, k_ptr, dist, rest):
+        out, low, lse = _lib.on_device(q.device, _launch, q, k, v, ptr, k_ptr, dist, slope, rest, True)
+        ctx.save_for_backward(q, k, v, slope, ptr, k_ptr, dist, out, low, lse)
+        ctx.rest = rest
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, grad_out):
-        L = _lib.load()
-        q, k, v, slope, ptr, k_ptr, dist, out, lse, low = ctx.saved_tensors
-        with torch.cuda.device(q.device):
-            grad_out = grad_out.contiguous()
-            if grad_out.data_ptr() % 16:
-                grad_out = grad_out.clone()
-            gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
-            gs = torch.empty_like(slope) if slope is not None and ctx.needs_input_grad[3] else None
-            a = _args(q, k, v, ptr, k_ptr, dist, slope, *ctx.rest)
-            a.out, a.lse, a.grad_out = out.data_ptr(), lse.data_ptr(), grad_out.data_ptr()
-            a.out_low = 0 if low is None else low.data_ptr()
-            a.grad_q, a.grad_k, a.grad_v = gq.data_ptr(), gk.data_ptr(), gv.data_ptr()
-            a.grad_slope = 0 if gs is None else gs.data_ptr()
-            need = L.trx_node_attention_workspace_bytes(a, 1)
-            ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
-            a.workspace, a.workspace_bytes = 0 if ws is None else ws.data_ptr(), need
-            _lib.check(L.trx_node_attention_backward(a, _lib.stream_ptr(q.device)), "trx_node_attention_backward")
-        return gq, gk, gv, gs, None, None, None, None, None, None, None, None
+        return *_lib.on_device(grad_out.device, _launch_backward, *ctx.saved_tensors, ctx.rest, grad_out,
+                               ctx.needs_input_grad[3]), None, None, None, None
 
 
 def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch.Tensor, *,
@@ -157,13 +157,14 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
     max_nodes = k.shape[0] if max_nodes is None else int(max_nodes)
     if max_queries < 0 or max_nodes < 0:
         raise ValueError(f"{what}: max_queries and max_nodes must be >= 0")
-    with _lib.on_device(what, q, k, v, ptr, k_ptr, dist, slope):
-        q, k, v, ptr, k_ptr = _strided(q), _strided(k), _strided(v), ptr.contiguous(), k_ptr.contiguous()
-        if dist is not None and dist.stride(-1) != 1:
-            dist = dist.contiguous()
-        if slope is not None:
-            slope = slope.contiguous()
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                        or (slope is not None and slope.requires_grad)):
-            return _NodeAttention.apply(q, k, v, slope, ptr, k_ptr, dist, scale, cap, max_queries, max_nodes, code)
-        return _forward(q, k, v, ptr, k_ptr, dist, slope, scale, cap, max_queries, max_nodes, code, False)[0]
+    _lib.same_device(what, q, k, v, ptr, k_ptr, dist, slope)
+    q, k, v, ptr, k_ptr = _strided(q), _strided(k), _strided(v), ptr.contiguous(), k_ptr.contiguous()
+    if dist is not None and dist.stride(-1) != 1:
+        dist = dist.contiguous()
+    if slope is not None:
+        slope = slope.contiguous()
+    rest = scale, cap, max_queries, max_nodes, code
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (slope is not None and slope.requires_grad)):
+        return _NodeAttention.apply(q, k, v, slope, ptr, k_ptr, dist, rest)
+    return _lib.on_device(q.device, _launch, q, k, v, ptr, k_ptr, dist, slope, rest, False)[0]

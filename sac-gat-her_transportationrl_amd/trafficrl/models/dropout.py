@@ -7,7 +7,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -17,38 +16,43 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _forward(x, residual, rng, border, site, code):
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    used = torch.empty(2, device=x.device, dtype=torch.int64)
-    _lib.check(_lib.load().trx_dropout_add_forward(x.numel(), code, _lib.ptr(x), _lib.ptr(residual), _lib.ptr(rng),
-                                                   border, site, _lib.ptr(y), _lib.ptr(used),
-                                                   _lib.stream_ptr(x.device)), "trx_dropout_add_forward")
+def _launch(x, residual, rng, rest, save: bool):
+    border, site, code = rest
+    y = torch.empty_like(x)
+    used = torch.empty_like(rng) if save else None
+    _lib.check(_lib.load().trx_dropout_add_forward(x.numel(), code, x.data_ptr(),
+                                                   None if residual is None else residual.data_ptr(), rng.data_ptr(),
+                                                   border, site, y.data_ptr(), None if used is None else used.data_ptr(),
+                                                   _lib.raw_stream(x.device)), "trx_dropout_add_forward")
     return y, used
+
+
+def _launch_backward(grad_y, used, rest):
+    border, site, code = rest
+    g = _aligned(grad_y)
+    grad_x = torch.empty_like(g)
+    _lib.check(_lib.load().trx_dropout_add_backward(g.numel(), code, g.data_ptr(), used.data_ptr(), border, site,
+                                                    grad_x.data_ptr(), _lib.raw_stream(g.device)),
+               "trx_dropout_add_backward")
+    return grad_x
 
 
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, rng, border, site, code):
-        with torch.cuda.device(x.device):
-            y, used = _forward(x, residual, rng, border, site, code)
+    def forward(ctx, x, residual, rng, rest):
+        y, used = _lib.on_device(x.device, _launch, x, residual, rng, rest, True)
         ctx.save_for_backward(used)
-        ctx.rest = border, site, code
+        ctx.rest = rest
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, grad_y):
-        used, = ctx.saved_tensors
-        border, site, code = ctx.rest
+        wants_x, wants_residual = ctx.needs_input_grad[:2]
         grad_x = None
-        if ctx.needs_input_grad[0]:
-            with torch.cuda.device(grad_y.device):
-                g = _aligned(grad_y)
-                grad_x = torch.empty(g.shape, device=g.device, dtype=g.dtype)
-                _lib.check(_lib.load().trx_dropout_add_backward(g.numel(), code, _lib.ptr(g), _lib.ptr(used), border,
-                                                                site, _lib.ptr(grad_x), _lib.stream_ptr(g.device)),
-                           "trx_dropout_add_backward")
-        return grad_x, grad_y if ctx.needs_input_grad[1] else None, None, None, None, None
+        if wants_x:
+            grad_x = _lib.on_device(grad_y.device, _launch_backward, grad_y, ctx.saved_tensors[0], ctx.rest)
+        return grad_x, grad_y if wants_residual else None, None, None
 
 
 def dropout_add(x: torch.Tensor, rng: torch.Tensor, p: float, *, residual: Optional[torch.Tensor] = None,
@@ -78,8 +82,10 @@ def dropout_add(x: torch.Tensor, rng: torch.Tensor, p: float, *, residual: Optio
         raise ValueError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} for x {tuple(x.shape)} {x.dtype}")
     if not 0 <= int(site) < 2 ** 32:
         raise ValueError(f"{what}: site must be 0 .. 2^32 - 1, got {site}")
-    with _lib.on_device(what, x, rng, residual):
-        x, rng, residual = _aligned(x), rng.contiguous(), None if residual is None else _aligned(residual)
-        if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-            return _DropoutAdd.apply(x, residual, rng, border, int(site), code)
-        return _forward(x, residual, rng, border, int(site), code)[0]
+    _lib.same_device(what, x, rng, residual)
+    x, rng, rest = _aligned(x), rng.contiguous(), (border, int(site), code)
+    if residual is not None:
+        residual = _aligned(residual)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _DropoutAdd.apply(x, residual, rng, rest)
+    return _lib.on_device(x.device, _launch, x, residual, rng, rest, False)[0]

@@ -6,9 +6,11 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
+
+
+_MASK_TYPES = (torch.float32, torch.bool, torch.uint8)
 
 
 class ActionLogProbs(NamedTuple):
@@ -18,68 +20,61 @@ class ActionLogProbs(NamedTuple):
     top_action: Optional[torch.Tensor]      # int64 [rows, top_k]
 
 
-def _args(logits, mask, row_ptr, action, max_row, top_k, code):
-    a = _lib.TrxActionLogProbsArgs()
-    a.dtype, a.top_k = code, top_k
+def _args(logits, mask, row_ptr, action, rest, outs, grads=(0, 0, 0, 0)):
+    max_row, top_k, code = rest
     if row_ptr is None:
-        a.rows, a.row_len, a.row_stride = logits.shape[0], logits.shape[1], logits.stride(0)
-        a.mask_stride = 0 if mask is None else mask.stride(0)
+        shape = (logits.shape[0], logits.shape[1], logits.stride(0), 0, 0, 0 if mask is None else mask.stride(0))
     else:
-        a.rows, a.total, a.max_row, a.row_ptr = row_ptr.numel() - 1, logits.numel(), max_row, row_ptr.data_ptr()
-    a.logits, a.action = logits.data_ptr(), action.data_ptr()
-    if mask is not None:
-        a.mask, a.mask_dtype = mask.data_ptr(), 0 if mask.dtype == torch.float32 else 1
-    return a
+        shape = (row_ptr.numel() - 1, 0, 0, logits.numel(), max_row, 0)
+    return _lib.TrxActionLogProbsArgs(
+        *shape, code, 0 if mask is None or mask.dtype == torch.float32 else 1, top_k, 0, logits.data_ptr(),
+        0 if mask is None else mask.data_ptr(), 0 if row_ptr is None else row_ptr.data_ptr(), action.data_ptr(),
+        *(0 if t is None else t.data_ptr() for t in outs), *grads)
 
 
-def _forward(logits, mask, row_ptr, action, max_row, top_k, code):
-    L = _lib.load()
-    a = _args(logits, mask, row_ptr, action, max_row, top_k, code)
-    n, dev = a.rows, logits.device
-    log_prob = torch.empty(n, device=dev)
-    entropy = torch.empty(n, device=dev)
-    stats = torch.empty(n, 4, device=dev)
+def _launch(logits, mask, row_ptr, action, rest):
+    L, top_k, dev = _lib.load(), rest[1], logits.device
+    n = action.shape[0]
+    log_prob, entropy, stats = torch.empty(n, device=dev), torch.empty(n, device=dev), torch.empty(n, 4, device=dev)
     top_log_prob = torch.empty(n, top_k, device=dev) if top_k else None
     top_action = torch.empty(n, top_k, device=dev, dtype=torch.int64) if top_k else None
-    a.log_prob, a.entropy, a.stats = log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
-    if top_k:
-        a.top_log_prob, a.top_action = top_log_prob.data_ptr(), top_action.data_ptr()
+    a = _args(logits, mask, row_ptr, action, rest, (log_prob, entropy, stats, top_log_prob, top_action))
     need = L.trx_action_log_probs_workspace_bytes(a)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need > 0 else None
-    a.workspace, a.workspace_bytes = 0 if ws is None else ws.data_ptr(), need
-    _lib.check(L.trx_action_log_probs_forward(a, _lib.stream_ptr(dev)), "trx_action_log_probs_forward")
+    ws = None
+    if need > 0:
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _lib.check(L.trx_action_log_probs_forward(a, _lib.raw_stream(dev)), "trx_action_log_probs_forward")
     return log_prob, entropy, top_log_prob, top_action, stats
+
+
+def _launch_backward(logits, mask, row_ptr, action, stats, top_action, rest, grads):
+    grads = [None if t is None else t.contiguous() for t in grads]
+    grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    a = _args(logits, mask, row_ptr, action, rest, (None, None, stats, None, top_action),
+              (*(0 if t is None else t.data_ptr() for t in grads), grad.data_ptr()))
+    _lib.check(_lib.load().trx_action_log_probs_backward(a, _lib.raw_stream(logits.device)),
+               "trx_action_log_probs_backward")
+    return grad
 
 
 class _ActionLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, mask, row_ptr, action, max_row, top_k, code):
-        with torch.cuda.device(logits.device):
-            log_prob, entropy, top_log_prob, top_action, stats = _forward(logits, mask, row_ptr, action, max_row, top_k,
-                                                                          code)
-        ctx.save_for_backward(logits, mask, row_ptr, action, log_prob, entropy, stats, top_action)
-        ctx.rest = max_row, top_k, code
+    def forward(ctx, logits, mask, row_ptr, action, rest):
+        *outs, stats = _lib.on_device(logits.device, _launch, logits, mask, row_ptr, action, rest)
+        ctx.save_for_backward(logits, mask, row_ptr, action, stats, outs[3])
+        ctx.rest = rest
         ctx.set_materialize_grads(False)
-        if top_k:
-            ctx.mark_non_differentiable(top_action)
-        return log_prob, entropy, top_log_prob, top_action
+        if outs[3] is not None:
+            ctx.mark_non_differentiable(outs[3])
+        return tuple(outs)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_log_prob, g_entropy, g_top, _g_action):
-        logits, mask, row_ptr, action, log_prob, entropy, stats, top_action = ctx.saved_tensors
-        max_row, top_k, code = ctx.rest
-        with torch.cuda.device(logits.device):
-            g = [None if t is None else t.contiguous() for t in (g_log_prob, g_entropy, g_top)]
-            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-            a = _args(logits, mask, row_ptr, action, max_row, top_k, code)
-            a.log_prob, a.entropy, a.stats = log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr()
-            a.top_action = 0 if top_action is None else top_action.data_ptr()
-            a.g_log_prob, a.g_entropy, a.g_top = (0 if t is None else t.data_ptr() for t in g)
-            a.grad_logits = grad.data_ptr()
-            _lib.check(_lib.load().trx_action_log_probs_backward(a, _lib.stream_ptr(logits.device)),
-                       "trx_action_log_probs_backward")
-        return grad, None, None, None, None, None, None
+    @_lib.once
+    def backward(ctx, *grads):
+        logits = ctx.saved_tensors[0]
+        return _lib.on_device(logits.device, _launch_backward, *ctx.saved_tensors, ctx.rest,
+                              grads[:3]), None, None, None, None
 
 
 def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Optional[torch.Tensor] = None,
@@ -126,16 +121,20 @@ def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Option
     if max_row < 0:
         raise ValueError(f"{what}: max_row must be >= 0")
     max_row = min(max_row, 2 ** 30)
-    with _lib.on_device(what, logits, action, mask, row_ptr):
-        if logits.numel() and logits.stride(-1) != 1:
-            logits = logits.contiguous()
-        action = action.long().contiguous()
-        if mask is not None:
-            if mask.dtype not in (torch.float32, torch.bool, torch.uint8):
-                mask = mask > 0
-            if mask.numel() and mask.stride(-1) != 1:
-                mask = mask.contiguous()
-        row_ptr = None if row_ptr is None else row_ptr.contiguous()
-        if torch.is_grad_enabled() and logits.requires_grad:
-            return ActionLogProbs(*_ActionLogProbs.apply(logits, mask, row_ptr, action, max_row, int(top_k), code))
-        return ActionLogProbs(*_forward(logits, mask, row_ptr, action, max_row, int(top_k), code)[:4])
+    _lib.same_device(what, logits, action, mask, row_ptr)
+    if logits.stride(-1) != 1 and logits.numel():
+        logits = logits.contiguous()
+    if action.dtype != torch.int64:
+        action = action.long()
+    action = action.contiguous()
+    if mask is not None:
+        if mask.dtype not in _MASK_TYPES:
+            mask = mask > 0
+        if mask.stride(-1) != 1 and mask.numel():
+            mask = mask.contiguous()
+    if row_ptr is not None:
+        row_ptr = row_ptr.contiguous()
+    rest = max_row, int(top_k), code
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return ActionLogProbs(*_ActionLogProbs.apply(logits, mask, row_ptr, action, rest))
+    return ActionLogProbs(*_lib.on_device(logits.device, _launch, logits, mask, row_ptr, action, rest)[:4])

@@ -179,7 +179,6 @@ def test_dropout_boundary():
     assert fwd(8, 0, 4096, None, 4096, 65536, 0, 4096, 4096, None) == -1
     assert fwd(8, 0, 4100, None, 4096, 1, 0, 4096, 4096, None) == -1
     assert fwd(8, 0, 4096, 4100, 4096, 1, 0, 4096, 4096, None) == -1
-    assert fwd(8, 0, 4096, None, 4096, 1, 0, 4096, None, None) == -1
     assert bwd(8, 0, 4096, 4096, -1, 0, 4096, None) == -1
     assert bwd(8, 0, 4096, None, 1, 0, 4096, None) == -1
     assert fwd(0, 0, None, None, None, 1, 0, None, None, None) == bwd(0, 0, None, None, 1, 0, None, None) == 0
