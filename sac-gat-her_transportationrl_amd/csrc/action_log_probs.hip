@@ -151,7 +151,7 @@ __device__ __forceinline__ void put_top(const Args& a, int64_t r, int k, uint64_
 
 // A row too long for the wave's registers (its length was not announced): passes over memory.
 template <typename T>
-__device__ __noinline__ void long_row(const Args& a, const Row& row, int64_t r, int lane) {
+__device__ __forceinline__ void long_row(const Args& a, const Row& row, int64_t r, int lane) {
     float m = -INFINITY;
     for (int64_t j = lane; j < row.len; j += kWave) m = fmaxf(m, logit<T>(a, row, j));
     uint64_t key = ~0ull;

@@ -55,6 +55,7 @@ __global__ void __launch_bounds__(kThreads)
             a = load8(x + e0);
             if (RES) b = load8(residual + e0);
         } else {
+#pragma unroll
             for (int e = 0; e < 8; ++e) {
                 a.e[e] = e < here ? x[e0 + e] : (T)0.0f;
                 if (RES) b.e[e] = e < here ? residual[e0 + e] : (T)0.0f;
@@ -71,7 +72,9 @@ __global__ void __launch_bounds__(kThreads)
         if (here == 8) {
             store8(y + e0, o);
         } else {
-            for (int e = 0; e < here; ++e) y[e0 + e] = o.e[e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < here) y[e0 + e] = o.e[e];
         }
     }
 }
