@@ -4,9 +4,9 @@
 //
 // With m = max x, s = sum e^(x - m) and t = sum e^(x - m) (x - m) over the links
 // that may be chosen: log p_j = x_j - m - log s and entropy = log s - t / s.
-// One read of the logits forward, one read and one write backward: rows of up
-// to 1024 links stay in one wave's registers, longer ones pass through a
-// workgroup's in chunks, split over several workgroups where there are few rows.
+// One read of the logits forward, one read and one write backward: rows pass
+// through registers, of one wave where they are short, of sixteen where they are
+// long, of several workgroups where there are few.
 // Ranking compares whole numbers made of the logit's bits and the link, so ties
 // go to the lower link whatever the order of anything.
 #include <hip/hip_runtime.h>
@@ -20,7 +20,7 @@ namespace trx {
 namespace {
 
 constexpr int kWave = 64;
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kThreads = kWave * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 using Args = trx_action_log_probs_args;
 
@@ -41,11 +41,25 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
     return max(max(at(0), at(16)), max(at(32), at(48)));
 }
-#undef TRX_DPP
 // the largest of the lanes' keys
 __device__ __forceinline__ uint64_t wave_max(uint64_t key) {
     const uint32_t high = (uint32_t)(key >> 32), top = wave_max(high);
     return ((uint64_t)top << 32) | wave_max(high == top ? (uint32_t)key : 0u);
+}
+
+// A number that at least `count` <= 16 of the lanes reach: the least of the maxima of 16, 8 or 4 groups of lanes
+__device__ __forceinline__ uint32_t reached_by(uint32_t v, int count) {
+    v = max(v, (uint32_t)TRX_DPP(v, 0xB1));
+    v = max(v, (uint32_t)TRX_DPP(v, 0x4E));            // 16 groups of four
+    if (count <= 8) v = max(v, (uint32_t)TRX_DPP(v, 0x141));
+    if (count <= 4) v = max(v, (uint32_t)TRX_DPP(v, 0x140));
+    return ~wave_max(~v);
+}
+#undef TRX_DPP
+// the lane's word for the whole wave
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
 // Whole numbers in the floats' order; 0 for -inf, NaN above +inf, the two zeros alike.
@@ -116,17 +130,10 @@ __device__ __forceinline__ void logits8(const Args& a, const Row& row, int64_t j
 struct Stats {
     float m, s, t;
 };
-__device__ __forceinline__ void add(Stats& x, float v, float m) {
+__device__ __forceinline__ void add(float& s, float& t, float v, float m) {
     const float d = v - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-    x.s += e;
-    x.t = __builtin_fmaf(e, fmaxf(d, -1e30f), x.t);   // where e is 0, d may be -inf
-}
-__device__ __forceinline__ Stats joined(const Stats& x, const Stats& y) {
-    if (x.m == -INFINITY && x.s == 0.0f) return y;
-    if (y.m == -INFINITY && y.s == 0.0f) return x;
-    const float m = fmaxf(x.m, y.m), dx = x.m - m, dy = y.m - m, fx = expf(dx), fy = expf(dy);
-    return {m, x.s * fx + y.s * fy,
-            fx * __builtin_fmaf(x.s, fmaxf(dx, -1e30f), x.t) + fy * __builtin_fmaf(y.s, fmaxf(dy, -1e30f), y.t)};
+    s += e;
+    t = __builtin_fmaf(e, fmaxf(d, -1e30f), t);   // where e is 0, d may be -inf
 }
 
 // a row's results from its statistics; one lane
@@ -149,40 +156,182 @@ __device__ __forceinline__ void put_top(const Args& a, int64_t r, int k, uint64_
     a.top_action[r * a.top_k + k] = key ? (int64_t)key_link(key) : -1;
 }
 
-// A row too long for the wave's registers (its length was not announced): passes over memory.
-template <typename T>
-__device__ __forceinline__ void long_row(const Args& a, const Row& row, int64_t r, int lane) {
-    float m = -INFINITY;
-    for (int64_t j = lane; j < row.len; j += kWave) m = fmaxf(m, logit<T>(a, row, j));
-    uint64_t key = ~0ull;
-    const uint32_t top = wave_max(order_of(m));
-    Stats x{top ? key_logit((uint64_t)top << 32) : -INFINITY, 0.0f, 0.0f};
-    for (int64_t j = lane; j < row.len; j += kWave) {
-        const float v = logit<T>(a, row, j);
-        if (v != -INFINITY) add(x, v, x.m == -INFINITY ? 0.0f : x.m);
+// Longer rows: a wave takes kPiece links at a time, two lots of eight consecutive ones a lane, and keeps running
+// statistics and its best top_k.  Nothing is shared between waves until the end.
+constexpr int kLots = 2, kPiece = kWave * 8 * kLots, kRoom = 64;
+
+struct Wave {
+    float m = -INFINITY;   // of the wave
+    float s = 0.0f, t = 0.0f;   // of the lane, around m
+    uint64_t kept = 0;     // lane k: the k-th best key
+};
+
+// The best top_k of up to 64 different keys in LDS, in order, one a lane: each lane counts the keys above its own.
+__device__ __forceinline__ uint64_t ranked(uint64_t* listed, int count, int top_k, int lane) {
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t key = lane < count ? listed[lane] : 0;
+    int above = 0;
+    for (int i = 0; i < count; ++i) above += from_lane(key, i) > key;
+    __builtin_amdgcn_wave_barrier();
+    if (lane < count && above < top_k) listed[above] = key;
+    __builtin_amdgcn_wave_barrier();
+    return lane < top_k && lane < count ? listed[lane] : 0;
+}
+// The same of N keys a lane (0: none): what reaches a bound that top_k lanes reach goes through the list; where too
+// many do, top_k rounds of the wave's maximum.
+template <int N>
+__device__ __forceinline__ uint64_t best_of(const uint64_t (&key)[N], uint64_t* listed, int top_k, int lane) {
+    uint32_t high = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) high = max(high, (uint32_t)(key[i] >> 32));
+    const uint32_t bound = max(reached_by(high, top_k), 1u);
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool in = (uint32_t)(key[i] >> 32) >= bound;
+        const uint64_t who = __ballot(in);
+        const int at = count + __popcll(who & ((1ull << lane) - 1));
+        if (in && at < kRoom) listed[at] = key[i];
+        count += __popcll(who);
     }
-    x.s = wave_sum(x.s);
-    x.t = wave_sum(x.t);
-    for (int k = 0; k < a.top_k; ++k) {
-        uint64_t next = 0;
-        for (int64_t j = lane; j < row.len && key; j += kWave) {
-            const uint64_t u = rank_key(logit<T>(a, row, j), (uint32_t)j);
-            if (u < key && u > next) next = u;
-        }
-        key = wave_max(next);
-        if (lane == 0) put_top(a, r, k, key, x);
+    if (count <= kRoom) return ranked(listed, count, top_k, lane);
+    uint64_t last = ~0ull, kept = 0;
+    for (int k = 0; k < top_k; ++k) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (key[i] < last && key[i] > best) best = key[i];
+        last = wave_max(best);
+        if (lane == k) kept = last;
     }
-    if (lane == 0) put_stats<T>(a, row, r, x);
+    return kept;
 }
 
-// one wave to a row of up to 64 V links
+// The alternatives are found by value first: of the lanes' own maxima, some bound is reached by at least top_k, and
+// few other logits of the piece reach it, so one comparison a logit leaves a short list in LDS.  Where many tie at
+// the bound, the wave takes its top_k one after the other from its registers instead.
+template <typename T>
+__device__ __forceinline__ void wave_pass(const Args& a, const Row& row, int64_t first, int64_t end, int64_t step,
+                                          int lane, uint64_t* listed, Wave& w) {
+    float x[kLots][8], next[kLots][8];
+    auto fetch = [&](int64_t j0) {
+#pragma unroll
+        for (int i = 0; i < kLots; ++i) logits8<T>(a, row, j0 + 8 * (lane + kWave * i), next[i]);
+    };
+    if (first < end) fetch(first);
+    for (int64_t j0 = first; j0 < end; j0 += step) {
+#pragma unroll
+        for (int i = 0; i < kLots; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = next[i][e];
+        if (j0 + step < end) fetch(j0 + step);
+        float mine = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kLots; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mine = fmaxf(mine, x[i][e]);
+        const uint32_t left = order_of(mine), top = wave_max(left);
+        const float m = top ? key_logit((uint64_t)top << 32) : -INFINITY;
+        if (m > w.m) {
+            const float d = w.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
+            w.t = f * __builtin_fmaf(w.s, fmaxf(d, -1e30f), w.t);
+            w.s *= f;
+            w.m = m;
+        }
+        const float base = w.m == -INFINITY ? 0.0f : w.m;
+#pragma unroll
+        for (int i = 0; i < kLots; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) add(w.s, w.t, x[i][e], base);
+        if (a.top_k == 0 || !top) continue;
+        // once top_k are kept, a logit has to pass the last of them: links only grow, so a tie loses
+        const uint64_t lowest = __shfl(w.kept, a.top_k - 1);
+        const float limit = lowest ? key_logit(lowest) : -INFINITY;
+        if (lowest && !(m > limit)) continue;
+        float reach = limit;
+        if (!lowest) {
+            const uint32_t bound = reached_by(left, a.top_k);
+            if (bound) reach = key_logit((uint64_t)bound << 32);
+        }
+        int count = 0;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kLots; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool in = x[i][e] >= reach && x[i][e] > limit;
+                const uint64_t who = __ballot(in);
+                if (who) {
+                    const int at = count + __popcll(who & ((1ull << lane) - 1));
+                    if (in && at < kRoom) listed[at] = rank_key(x[i][e], (uint32_t)(j0 + 8 * (lane + kWave * i) + e));
+                    count += __popcll(who);
+                }
+            }
+        if (lowest && count <= a.top_k) {   // few: each goes in at its place
+            __builtin_amdgcn_wave_barrier();
+            const uint64_t fresh = lane < count ? listed[lane] : 0;
+            for (int i = 0; i < count; ++i) {
+                const uint64_t key = from_lane(fresh, i), before = __shfl_up(w.kept, 1);
+                const int at = __popcll(__ballot(w.kept > key));
+                if (lane >= at && lane < a.top_k) w.kept = lane == at ? key : before;
+            }
+        } else if (count + a.top_k <= kRoom) {
+            const uint64_t old = __ballot(w.kept != 0);   // the lanes from 0 on
+            if (w.kept) listed[count + lane] = w.kept;
+            w.kept = ranked(listed, count + __popcll(old), a.top_k, lane);
+        } else {
+            const uint64_t old = w.kept;
+            uint64_t last = ~0ull;
+            for (int k = 0; k < a.top_k; ++k) {
+                uint64_t best = old < last ? old : 0;
+#pragma unroll
+                for (int i = 0; i < kLots; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint64_t key = rank_key(x[i][e], (uint32_t)(j0 + 8 * (lane + kWave * i) + e));
+                        if (key < last && key > best) best = key;
+                    }
+                last = wave_max(best);
+                if (lane == k) w.kept = last;
+            }
+        }
+    }
+}
+
+// the best top_k of some of a row's links by their keys alone, passes over memory: for rows in which a NaN ranks
+template <typename T>
+__device__ __forceinline__ uint64_t ranked_by_keys(const Args& a, const Row& row, int64_t first, int64_t end, int lane) {
+    uint64_t kept = 0, last = ~0ull;
+    for (int k = 0; k < a.top_k && last; ++k) {
+        uint64_t best = 0;
+        for (int64_t j = first + lane; j < end; j += kWave) {
+            const uint64_t key = rank_key(logit<T>(a, row, j), (uint32_t)j);
+            if (key < last && key > best) best = key;
+        }
+        last = wave_max(best);
+        if (lane == k) kept = last;
+    }
+    return kept;
+}
+
+// One wave to a row.  Up to 64 V links: a link a lane at a time, all ranked by keys; more: in pieces.  At 76 links the
+// pieces' eight a lane would leave five lanes of six idle.
 template <typename T, int V>
 __global__ void __launch_bounds__(kWave * kWaves) log_probs_short_kernel(Args a) {
-    const int lane = threadIdx.x % kWave;
-    const int64_t r = (int64_t)blockIdx.x * kWaves + threadIdx.x / kWave;
+    __shared__ uint64_t listed[kWaves][kRoom];
+    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+    const int64_t r = (int64_t)blockIdx.x * kWaves + w;
     if (r >= a.rows) return;
     const Row row = find_row(a, r);
-    if (row.len > kWave * V) return long_row<T>(a, row, r, lane);
+    if (row.len > kWave * V) {
+        Wave x;
+        wave_pass<T>(a, row, 0, row.len, kPiece, lane, listed[w], x);
+        const Stats st{x.m, wave_sum(x.s), wave_sum(x.t)};
+        if (st.s != st.s) x.kept = ranked_by_keys<T>(a, row, 0, row.len, lane);
+        if (lane < a.top_k) put_top(a, r, lane, x.kept, st);
+        if (lane == 0) put_stats<T>(a, row, r, st);
+        return;
+    }
     const int n = (int)row.len;
     float x[V];
 #pragma unroll
@@ -194,25 +343,17 @@ __global__ void __launch_bounds__(kWave * kWaves) log_probs_short_kernel(Args a)
     Stats st{top ? key_logit((uint64_t)top << 32) : -INFINITY, 0.0f, 0.0f};
     const float base = top ? st.m : 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) add(st, x[i], base);
+    for (int i = 0; i < V; ++i) add(st.s, st.t, x[i], base);
     st.s = wave_sum(st.s);
     st.t = wave_sum(st.t);
     if (lane == 0) put_stats<T>(a, row, r, st);
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.top_k; ++k) {
-        uint64_t best = 0;
+    if (a.top_k == 0) return;
+    uint64_t key[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const uint64_t key = rank_key(x[i], lane + kWave * i);
-            if (key < last && key > best) best = key;
-        }
-        last = wave_max(best);
-        if (lane == 0) put_top(a, r, k, last, st);
-    }
+    for (int i = 0; i < V; ++i) key[i] = rank_key(x[i], lane + kWave * i);
+    const uint64_t kept = best_of(key, listed[w], a.top_k, lane);
+    if (lane < a.top_k) put_top(a, r, lane, kept, st);
 }
-
-// Longer rows: a workgroup holds kChunk links at a time, 32 a thread.
-constexpr int kEach = 4, kThreads = kWave * kWaves, kChunk = kThreads * 8 * kEach, kRoom = 64;
 
 struct Parts {
     float4* stats;     // [rows, slots]: m, s, t
@@ -222,150 +363,78 @@ __device__ __forceinline__ Parts parts_of(const Args& a, int slots) {
     float4* s = static_cast<float4*>(a.workspace);
     return {s, reinterpret_cast<uint64_t*>(s + a.rows * slots)};
 }
+// one wave: the lanes' statistics as one
+__device__ __forceinline__ Stats joined(float m, float s, float t) {
+    const uint32_t top = wave_max(order_of(m));
+    const float all = top ? key_logit((uint64_t)top << 32) : -INFINITY, d = m == -INFINITY ? 0.0f : m - all;
+    const float f = expf(d);
+    return {all, wave_sum(s * f), wave_sum(f * __builtin_fmaf(s, d, t))};
+}
 
-// The alternatives are found by value first: the top_k-th largest of the lanes' own maxima is a bound that at least
-// top_k of the wave's logits reach, and few others do, so one comparison a logit leaves a short list in LDS.  Where
-// many tie at the bound, or a NaN ranks, the wave takes its top_k one after the other from its registers instead.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) log_probs_long_kernel(Args a, int slots) {
-    __shared__ uint64_t listed[kWaves][kRoom], kept[TRX_TOP_MAX];
-    __shared__ float red[3][kWaves];
+// W waves to a row, or to one of its slots: consecutive `each` links (a multiple of kPiece)
+template <typename T, int W>
+__global__ void __launch_bounds__(kWave * W) log_probs_long_kernel(Args a, int slots) {
+    __shared__ uint64_t listed[W][kRoom], lists[W * TRX_TOP_MAX];
+    __shared__ float red[3][W];
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
     const int64_t r = blockIdx.x;
     const Row row = find_row(a, r);
-    Stats all{-INFINITY, 0.0f, 0.0f};
-    if (threadIdx.x < TRX_TOP_MAX) kept[threadIdx.x] = 0;
-    for (int64_t j0 = (int64_t)blockIdx.y * kChunk; j0 < row.len; j0 += (int64_t)slots * kChunk) {
-        float x[kEach][8];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) logits8<T>(a, row, j0 + 8 * (threadIdx.x + kThreads * i), x[i]);
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, x[i][e]);
-        const uint32_t mine = order_of(m), wave_top = wave_max(mine);
-        const float base = wave_top ? key_logit((uint64_t)wave_top << 32) : 0.0f;
-        Stats st{wave_top ? base : -INFINITY, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) add(st, x[i][e], base);
-        st.s = wave_sum(st.s);
-        st.t = wave_sum(st.t);
-        if (a.top_k > 0) {
-            uint32_t left = mine, bound = 0;
-            for (int k = 0; k < a.top_k; ++k) {
-                bound = wave_max(left);
-                if (!bound) break;
-                // one lane of the maximum is done with
-                const uint64_t who = __ballot(left == bound);
-                if (lane == __ffsll((unsigned long long)who) - 1) left = 0;
-            }
-            int count = 0;
-            bool fits = st.s == st.s;   // a NaN: by keys
-            if (fits && wave_top) {
-                const float limit = bound ? key_logit((uint64_t)bound << 32) : -INFINITY;
-#pragma unroll
-                for (int i = 0; i < kEach; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const bool in = x[i][e] >= limit && x[i][e] > -INFINITY;
-                        const uint64_t who = __ballot(in);
-                        if (who) {
-                            const int at = count + __popcll(who & ((1ull << lane) - 1));
-                            if (in && at < kRoom)
-                                listed[w][at] = rank_key(x[i][e], (uint32_t)(j0 + 8 * (threadIdx.x + kThreads * i) + e));
-                            count += __popcll(who);
-                        }
-                    }
-                fits = count <= kRoom;
-            }
-            if (!fits) {
-                uint64_t last = ~0ull;
-                count = 0;
-                for (int k = 0; k < a.top_k && last; ++k) {
-                    uint64_t best = 0;
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint64_t key = rank_key(x[i][e], (uint32_t)(j0 + 8 * (threadIdx.x + kThreads * i) + e));
-                            if (key < last && key > best) best = key;
-                        }
-                    last = wave_max(best);
-                    if (last) {
-                        if (lane == 0) listed[w][k] = last;
-                        count = k + 1;
-                    }
-                }
-            }
-            if (lane >= count) listed[w][lane] = 0;
-        }
-        if (lane == 0) {
-            red[0][w] = st.m;
-            red[1][w] = st.s;
-            red[2][w] = st.t;
-        }
-        __syncthreads();
-        // every thread of wave 0 joins the waves' statistics; their lists and what was kept so far become top_k again
-        if (w == 0) {
-#pragma unroll
-            for (int v = 0; v < kWaves; ++v) all = joined(all, Stats{red[0][v], red[1][v], red[2][v]});
-            if (a.top_k > 0) {
-                uint64_t key[kWaves + 1];
-#pragma unroll
-                for (int v = 0; v < kWaves; ++v) key[v] = listed[v][lane];
-                key[kWaves] = lane < TRX_TOP_MAX ? kept[lane] : 0;
-                uint64_t last = ~0ull, mine_kept = 0;
-                for (int k = 0; k < a.top_k; ++k) {
-                    uint64_t best = 0;
-#pragma unroll
-                    for (int v = 0; v <= kWaves; ++v)
-                        if (key[v] < last && key[v] > best) best = key[v];
-                    last = wave_max(best);
-                    if (lane == k) mine_kept = last;
-                }
-                if (lane < TRX_TOP_MAX) kept[lane] = lane < a.top_k ? mine_kept : 0;
-            }
-        }
-        __syncthreads();
+    const int64_t each = ((row.len + kPiece - 1) / kPiece + slots - 1) / slots * kPiece;
+    const int64_t first = min(row.len, blockIdx.y * each), end = min(row.len, first + each);
+    Wave x;
+    wave_pass<T>(a, row, first + w * kPiece, end, W * kPiece, lane, listed[w], x);
+    x.s = wave_sum(x.s);
+    x.t = wave_sum(x.t);
+    if (lane < TRX_TOP_MAX) lists[w * TRX_TOP_MAX + lane] = lane < a.top_k ? x.kept : 0;
+    if (lane == 0) {
+        red[0][w] = x.m;
+        red[1][w] = x.s;
+        red[2][w] = x.t;
     }
+    __syncthreads();
     if (w != 0) return;
+    const bool has = lane < W;
+    const Stats st = joined(has ? red[0][lane] : -INFINITY, has ? red[1][lane] : 0.0f, has ? red[2][lane] : 0.0f);
+    if (a.top_k > 0) {
+        if (st.s != st.s) {
+            x.kept = ranked_by_keys<T>(a, row, first, end, lane);
+        } else {
+            constexpr int kLists = (W * TRX_TOP_MAX + kWave - 1) / kWave;
+            uint64_t key[kLists];
+#pragma unroll
+            for (int i = 0; i < kLists; ++i) key[i] = lists[lane + kWave * i];
+            x.kept = best_of(key, listed[0], a.top_k, lane);
+        }
+    }
     if (slots == 1) {
-        if (lane < a.top_k) put_top(a, r, lane, kept[lane], all);
-        if (lane == 0) put_stats<T>(a, row, r, all);
+        if (lane < a.top_k) put_top(a, r, lane, x.kept, st);
+        if (lane == 0) put_stats<T>(a, row, r, st);
     } else {
         const Parts p = parts_of(a, slots);
         const int64_t at = r * slots + blockIdx.y;
-        if (lane == 0) p.stats[at] = make_float4(all.m, all.s, all.t, 0.0f);
-        if (lane < a.top_k) p.keys[at * a.top_k + lane] = kept[lane];
+        if (lane == 0) p.stats[at] = make_float4(st.m, st.s, st.t, 0.0f);
+        if (lane < a.top_k) p.keys[at * a.top_k + lane] = x.kept;
     }
 }
 
-// one wave to a row: its slots' statistics in their order, their sorted alternatives merged
+// one wave to a row: the statistics of its slots (at most 64), their alternatives merged
 template <typename T>
 __global__ void __launch_bounds__(kWave * kWaves) log_probs_join_kernel(Args a, int slots) {
+    __shared__ uint64_t listed[kWaves][kRoom];
     const int lane = threadIdx.x % kWave;
     const int64_t r = (int64_t)blockIdx.x * kWaves + threadIdx.x / kWave;
     if (r >= a.rows) return;
     const Parts p = parts_of(a, slots);
-    Stats x{-INFINITY, 0.0f, 0.0f};
-    for (int s = 0; s < slots; ++s) {
-        const float4 v = p.stats[r * slots + s];
-        x = joined(x, Stats{v.x, v.y, v.z});
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.top_k; ++k) {
-        uint64_t best = 0;
-        for (int i = lane; i < slots * a.top_k; i += kWave) {
-            const uint64_t key = p.keys[r * slots * a.top_k + i];
-            if (key < last && key > best) best = key;
-        }
-        last = wave_max(best);
-        if (lane == 0) put_top(a, r, k, last, x);
-    }
-    if (lane == 0) put_stats<T>(a, find_row(a, r), r, x);
+    const float4 v = lane < slots ? p.stats[r * slots + lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    const Stats st = joined(v.x, v.y, v.z);
+    constexpr int kLists = TRX_TOP_MAX;   // 64 slots' lists over 64 lanes
+    uint64_t key[kLists], kept = 0;
+#pragma unroll
+    for (int i = 0; i < kLists; ++i)
+        key[i] = lane + kWave * i < slots * a.top_k ? p.keys[r * slots * a.top_k + lane + kWave * i] : 0;
+    if (a.top_k > 0) kept = best_of(key, listed[threadIdx.x / kWave], a.top_k, lane);
+    if (lane < a.top_k) put_top(a, r, lane, kept, st);
+    if (lane == 0) put_stats<T>(a, find_row(a, r), r, st);
 }
 
 // ---------------------------------------------------------------- backward
@@ -443,7 +512,8 @@ __global__ void __launch_bounds__(kWave * kWaves) log_probs_short_bwd_kernel(Arg
     }
 }
 
-// a workgroup to a chunk of a row, eight links a lane at a time
+// a workgroup to kChunk links of a row at a time, four lots of eight a lane
+constexpr int kEach = 4, kChunk = kThreads * 8 * kEach;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) log_probs_long_bwd_kernel(Args a) {
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
@@ -487,20 +557,22 @@ __global__ void __launch_bounds__(kThreads) log_probs_long_bwd_kernel(Args a) {
     }
 }
 
-// up to here one wave holds a row: 16 links a lane
-constexpr int kShort = 16 * kWave;
-
 int64_t longest(const Args& a) { return a.row_ptr ? a.max_row : a.row_len; }
-// workgroups to a long row: as many as fill the chip four times, but no more than it has chunks
+
+// Waves to a row: one up to 1024 links (four such rows a workgroup), four up to 8192 or where a thousand rows fill the
+// chip by themselves (each wave finds its first alternatives anew, so fewer waves do less), sixteen beyond.  Rows are
+// split into slots where they alone would leave compute units idle, each of at least sixteen pieces (a slot costs its
+// part of the joining launch).
+constexpr int kOneWave = kPiece, kFourWaves = 8 * kPiece, kManyRows = 1024;
 int slots_of(const Args& a) {
-    const int64_t chunks = (longest(a) + kChunk - 1) / kChunk, want = (1024 + a.rows - 1) / std::max<int64_t>(1, a.rows);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(chunks, want), 1024));
+    const int64_t n = longest(a), pieces = (n + kPiece - 1) / kPiece, rows = std::max<int64_t>(1, a.rows);
+    if (n <= kFourWaves || rows >= kManyRows) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pieces / 16, 64), 256 / rows));
 }
 
 }  // namespace
 
 size_t action_log_probs_workspace(const trx_action_log_probs_args& a) {
-    if (longest(a) <= kShort) return 0;
     const int slots = slots_of(a);
     return slots > 1 ? (size_t)a.rows * slots * (sizeof(float4) + a.top_k * sizeof(uint64_t)) : 0;
 }
@@ -509,15 +581,16 @@ hipError_t launch_action_log_probs_fwd(const trx_action_log_probs_args& a, hipSt
     return by_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const int64_t n = longest(a);
-        const dim3 by_four((unsigned)((a.rows + kWaves - 1) / kWaves)), block(kThreads);
-        if (n <= 2 * kWave) {
-            hipLaunchKernelGGL((log_probs_short_kernel<T, 2>), by_four, block, 0, stream, a);
-        } else if (n <= kShort) {
-            hipLaunchKernelGGL((log_probs_short_kernel<T, kShort / kWave>), by_four, block, 0, stream, a);
+        const dim3 by_four((unsigned)((a.rows + kWaves - 1) / kWaves)), by_one((unsigned)a.rows);
+        const int slots = slots_of(a);
+        if (n <= kOneWave) {
+            hipLaunchKernelGGL((log_probs_short_kernel<T, 2>), by_four, dim3(kThreads), 0, stream, a);
+        } else if (n <= kFourWaves || a.rows >= kManyRows) {
+            hipLaunchKernelGGL((log_probs_long_kernel<T, 4>), by_one, dim3(kThreads), 0, stream, a, 1);
         } else {
-            const int slots = slots_of(a);
-            hipLaunchKernelGGL(log_probs_long_kernel<T>, dim3((unsigned)a.rows, slots), block, 0, stream, a, slots);
-            if (slots > 1) hipLaunchKernelGGL(log_probs_join_kernel<T>, by_four, block, 0, stream, a, slots);
+            hipLaunchKernelGGL((log_probs_long_kernel<T, 16>), dim3((unsigned)a.rows, slots), dim3(16 * kWave), 0, stream,
+                               a, slots);
+            if (slots > 1) hipLaunchKernelGGL(log_probs_join_kernel<T>, by_four, dim3(kThreads), 0, stream, a, slots);
         }
         return hipGetLastError();
     });
@@ -527,7 +600,7 @@ hipError_t launch_action_log_probs_bwd(const trx_action_log_probs_args& a, hipSt
     return by_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const int64_t n = longest(a);
-        if (n <= kShort) {
+        if (n <= kOneWave) {
             const int blocks = (int)((a.rows + kWaves - 1) / kWaves), rest = a.row_ptr ? 16 : 0;
             hipLaunchKernelGGL(log_probs_short_bwd_kernel<T>, dim3(blocks + rest), dim3(kThreads), 0, stream, a, blocks);
         } else {
