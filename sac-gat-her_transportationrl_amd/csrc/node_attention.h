@@ -159,6 +159,52 @@ inline Call call_of(const Args& a, int64_t tiles) {
             (int)tiles * units};
 }
 
+// ROWS query rows' distances to KT keys, through registers to LDS like the tiles.  A fragment's lanes hold sixteen
+// rows side by side, so reading them where they are used would touch sixteen cache lines for every sixteen lanes;
+// here the lanes run along the rows.
+template <int ROWS, int KT, int THREADS>
+struct StagedDistances {
+    static constexpr int kLanes = KT / 4, kStep = THREADS / kLanes, kEach = ROWS / kStep, kPitch = KT + 4;
+    f32x4 r[kEach];
+
+    // rows row0 .. row0 + ROWS of the graph's (query, head of the group)s, `rows` of them there; keys from j on
+    __device__ __forceinline__ void load(const Call& call, const float* graph, int row0, int rows, int keys, int j) {
+        const Args& a = call.a;
+        const int G = call.group.by, mine = threadIdx.x / kLanes, col = 4 * (threadIdx.x % kLanes);
+        const int limit = min(keys, a.dist_cols), i0 = call.group(row0);
+        // rows in equal steps and all there: one 32-bit offset a lane, the rest is scalar
+        if (row0 + ROWS <= rows && call.group(row0 + ROWS - 1) < a.dist_rows && j + KT <= limit && 16 % G == 0 &&
+            kStep % G == 0 && row0 % G == 0 && a.dist_row < (1 << 24)) {
+            const float* base = graph + i0 * a.dist_row + j;
+            const uint32_t off = call.group(mine) * (uint32_t)a.dist_row + col;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e)
+                r[e] = *reinterpret_cast<const f32x4u*>(base + e * (kStep / G) * a.dist_row + off);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int row = row0 + mine + kStep * e, i = call.group(min(row, rows - 1));
+            const float* p = graph + i * a.dist_row + j + col;
+            const int left = i < a.dist_rows ? limit - j - col : 0;
+            f32x4 v{INFINITY, INFINITY, INFINITY, INFINITY};
+            if (left >= 4) {
+                v = *reinterpret_cast<const f32x4u*>(p);
+            } else if (left > 0) {
+                v[0] = p[0];
+                if (left > 1) v[1] = p[1];
+                if (left > 2) v[2] = p[2];
+            }
+            r[e] = v;
+        }
+    }
+    __device__ __forceinline__ void store(float* tile) const {
+        const int mine = threadIdx.x / kLanes, col = 4 * (threadIdx.x % kLanes);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) *reinterpret_cast<f32x4*>(tile + (mine + kStep * e) * kPitch + col) = r[e];
+    }
+};
+
 // four elements of a result; where `low` is given, what rounding took from them goes there
 template <typename T>
 __device__ __forceinline__ void put4(T* out, T* low, int64_t at, f32x4 v) {

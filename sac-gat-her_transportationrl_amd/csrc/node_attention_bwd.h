@@ -26,6 +26,9 @@ __global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_
 attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
     constexpr bool kAhead = WAVES > 1;   // one wave's registers are better spent on more waves
+    constexpr bool kStageD = DIST && WAVES > 1;
+    using Distances = StagedDistances<kStageD ? kRows : kTiles * 16, KT, kThreads>;
+    __shared__ __attribute__((aligned(16))) float d_tile[kStageD ? kRows * Distances::kPitch : 4];
     __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
@@ -88,7 +91,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
             }
             D[t] = column_sum(dot);
             bias[t] = bias_of<DIST, CAP>(a, DIST && a.slope ? a.slope[h] : 0.0f);
-            if (DIST) {
+            if (DIST && !kStageD) {
                 dist[t] = a.dist + b * a.dist_graph + i * a.dist_row;
                 limit[t] = i < a.dist_rows ? min(ks.n, a.dist_cols) : 0;
             }
@@ -99,10 +102,13 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) acc[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        f32x4 d[MQ][kTiles];
+        const float* graph = DIST ? a.dist + b * a.dist_graph : nullptr;
+        Distances d_next;
+        if (kStageD && first < last) d_next.load(call, graph, tile * kRows, rows, ks.n, first);
         for (int j0 = first; j0 < last; j0 += KT) {
+            f32x4 d[MQ][kTiles];
             if (!kAhead) fetch(j0);
-            if (DIST && row0 < rows) {
+            if (DIST && !kStageD) {
 #pragma unroll
                 for (int t = 0; t < MQ; ++t) {
                     const bool whole = __all(j0 + KT <= limit[t]);
@@ -113,8 +119,12 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
             __syncthreads();
             k_next.store(k_tile);
             v_next.store(v_tile);
+            if (kStageD) d_next.store(d_tile);
             __syncthreads();
-            if (kAhead && j0 + KT < last) fetch(j0 + KT);
+            if (kAhead && j0 + KT < last) {
+                fetch(j0 + KT);
+                if (kStageD) d_next.load(call, graph, tile * kRows, rows, ks.n, j0 + KT);
+            }
             if (row0 >= rows) continue;
             f32x4 s[MQ][kTiles], gp[MQ][kTiles];
 #pragma unroll
@@ -137,6 +147,12 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
             frag<T> u[MQ][KT / 32];
 #pragma unroll
             for (int t = 0; t < MQ; ++t) {
+                if (kStageD) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+                        d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + (w * 16 * MQ + 16 * t + c) * Distances::kPitch +
+                                                                  16 * n + 4 * g);
+                }
                 const bool cut = !DIST && j0 + KT > last, free = DIST && __all(bias[t].slope < 0.0f) && ordinary(d[t]);
                 const float slope = bias[t].slope, unit = bias[t].unit;
 #pragma unroll

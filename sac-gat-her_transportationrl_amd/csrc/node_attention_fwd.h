@@ -19,7 +19,9 @@ __global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_
 attention_fwd_kernel(Call call, float* part) {
     constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
     constexpr bool kAhead = WAVES > 1;   // one wave's registers are better spent on more waves
-    constexpr bool kAheadD = kAhead && CP == 128;   // registers for the next tile's distances: at 64 channels they cost more than they hide
+    constexpr bool kStageD = DIST && WAVES > 1;
+    using Distances = StagedDistances<kStageD ? kRows : kTiles * 16, KT, kThreads>;
+    __shared__ __attribute__((aligned(16))) float d_tile[kStageD ? kRows * Distances::kPitch : 4];
     __shared__ __attribute__((aligned(16))) T k_tile[KT * kRow<T, CP>], v_tile[KT * kRow<T, CP>];
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
@@ -64,7 +66,7 @@ attention_fwd_kernel(Call call, float* part) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) q[t][s] = 32 * s + 8 * g < C ? load_frag(p + 32 * s + 8 * g) : zero_frag<T>();
             bias[t] = bias_of<DIST, CAP>(a, DIST && a.slope ? a.slope[h] : 0.0f);
-            if (DIST) {
+            if (DIST && !kStageD) {
                 dist[t] = a.dist + b * a.dist_graph + i * a.dist_row;
                 limit[t] = i < a.dist_rows ? min(ks.n, a.dist_cols) : 0;
             }
@@ -73,30 +75,28 @@ attention_fwd_kernel(Call call, float* part) {
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) o[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        f32x4 d[MQ][kTiles], d_next[MQ][kTiles];
-        auto fetch_distances = [&](int j0, f32x4(&to)[MQ][kTiles]) {
-#pragma unroll
-            for (int t = 0; t < MQ; ++t) {
-                const bool whole = __all(j0 + KT <= limit[t]);
-#pragma unroll
-                for (int n = 0; n < kTiles; ++n) to[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
-            }
-        };
-        if (DIST && kAheadD && first < last && row0 < rows) fetch_distances(first, d_next);
+        const float* graph = DIST ? a.dist + b * a.dist_graph : nullptr;
+        Distances d_next;
+        if (kStageD && first < last) d_next.load(call, graph, tile * kRows, rows, ks.n, first);
         for (int j0 = first; j0 < last; j0 += KT) {
+            f32x4 d[MQ][kTiles];
             if (!kAhead) fetch(j0);
-            if (DIST && !kAheadD && row0 < rows) fetch_distances(j0, d);
+            if (DIST && !kStageD) {
+#pragma unroll
+                for (int t = 0; t < MQ; ++t) {
+                    const bool whole = __all(j0 + KT <= limit[t]);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) d[t][n] = distances(dist[t], j0 + 16 * n + 4 * g, limit[t], whole);
+                }
+            }
             __syncthreads();
             k_next.store(k_tile);
             v_next.store(v_tile);
+            if (kStageD) d_next.store(d_tile);
             __syncthreads();
-            if (kAhead && j0 + KT < last) fetch(j0 + KT);
-            if (DIST && kAheadD && row0 < rows) {
-#pragma unroll
-                for (int t = 0; t < MQ; ++t)
-#pragma unroll
-                    for (int n = 0; n < kTiles; ++n) d[t][n] = d_next[t][n];
-                if (j0 + KT < last) fetch_distances(j0 + KT, d_next);
+            if (kAhead && j0 + KT < last) {
+                fetch(j0 + KT);
+                if (kStageD) d_next.load(call, graph, tile * kRows, rows, ks.n, j0 + KT);
             }
             if (row0 >= rows) continue;
             f32x4 s[MQ][kTiles];
@@ -114,6 +114,12 @@ attention_fwd_kernel(Call call, float* part) {
             frag<T> p[MQ][KT / 32];
 #pragma unroll
             for (int t = 0; t < MQ; ++t) {
+                if (kStageD) {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+                        d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + (w * 16 * MQ + 16 * t + c) * Distances::kPitch +
+                                                                  16 * n + 4 * g);
+                }
                 // scores in bias.unit, and their maximum
 #define EACH_SCORE                  \
     _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
