@@ -159,43 +159,64 @@ inline Call call_of(const Args& a, int64_t tiles) {
             (int)tiles * units};
 }
 
+// one column's four distances behind key j: +inf from `limit` on
+__device__ __forceinline__ f32x4 distances(const float* row, int j, int limit, bool whole) {
+    if (whole || j + 4 <= limit) return *reinterpret_cast<const f32x4u*>(row + j);
+    f32x4 d{INFINITY, INFINITY, INFINITY, INFINITY};
+    if (j < limit) {
+        d[0] = row[j];
+        if (j + 1 < limit) d[1] = row[j + 1];
+        if (j + 2 < limit) d[2] = row[j + 2];
+    }
+    return d;
+}
+
 // ROWS query rows' distances to KT keys, through registers to LDS like the tiles.  A fragment's lanes hold sixteen
 // rows side by side, so reading them where they are used would touch sixteen cache lines for every sixteen lanes;
 // here the lanes run along the rows.
+//
+// Where rows go in equal steps, one 32-bit offset a lane and scalars address them all.  The last tile's window then
+// ends at the matrix's last row and key instead of passing them: `shift` is how far its rows lie behind where the
+// tile's first row would be (rows behind the last that is read meet nothing), and lanes that were moved back along
+// the keys move their values.  Every other shape takes each row by itself.
 template <int ROWS, int KT, int THREADS>
 struct StagedDistances {
     static constexpr int kLanes = KT / 4, kStep = THREADS / kLanes, kEach = ROWS / kStep, kPitch = KT + 4;
     f32x4 r[kEach];
+    int shift;
 
     // rows row0 .. row0 + ROWS of the graph's (query, head of the group)s, `rows` of them there; keys from j on
     __device__ __forceinline__ void load(const Call& call, const float* graph, int row0, int rows, int keys, int j) {
         const Args& a = call.a;
         const int G = call.group.by, mine = threadIdx.x / kLanes, col = 4 * (threadIdx.x % kLanes);
-        const int limit = min(keys, a.dist_cols), i0 = call.group(row0);
-        // rows in equal steps and all there: one 32-bit offset a lane, the rest is scalar
-        if (row0 + ROWS <= rows && call.group(row0 + ROWS - 1) < a.dist_rows && j + KT <= limit && 16 % G == 0 &&
-            kStep % G == 0 && row0 % G == 0 && a.dist_row < (1 << 24)) {
-            const float* base = graph + i0 * a.dist_row + j;
-            const uint32_t off = call.group(mine) * (uint32_t)a.dist_row + col;
+        const int limit = min(keys, a.dist_cols), i0 = call.group(row0), end = min(row0 + ROWS, rows);
+        const int first = min(i0, a.dist_rows - ROWS / G);
+        shift = 0;
+        if (kStep % G == 0 && row0 % G == 0 && a.dist_row < (1 << 24) && limit >= 4 && first >= 0 &&
+            call.group(end - 1) < a.dist_rows) {
+            shift = (i0 - first) * G;
+            const int j1 = min(j, limit - 4), at = min(j + col, limit - 4), back = j + col - at;
+            const float* base = graph + first * a.dist_row + j1;
+            const uint32_t off = call.group(mine) * (uint32_t)a.dist_row + (at - j1);
 #pragma unroll
             for (int e = 0; e < kEach; ++e)
                 r[e] = *reinterpret_cast<const f32x4u*>(base + e * (kStep / G) * a.dist_row + off);
+            if (j + KT > limit) {
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const f32x4 v = r[e];
+                    r[e][0] = back == 0 ? v[0] : back == 1 ? v[1] : back == 2 ? v[2] : back == 3 ? v[3] : INFINITY;
+                    r[e][1] = back == 0 ? v[1] : back == 1 ? v[2] : back == 2 ? v[3] : INFINITY;
+                    r[e][2] = back == 0 ? v[2] : back == 1 ? v[3] : INFINITY;
+                    r[e][3] = back == 0 ? v[3] : INFINITY;
+                }
+            }
             return;
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             const int row = row0 + mine + kStep * e, i = call.group(min(row, rows - 1));
-            const float* p = graph + i * a.dist_row + j + col;
-            const int left = i < a.dist_rows ? limit - j - col : 0;
-            f32x4 v{INFINITY, INFINITY, INFINITY, INFINITY};
-            if (left >= 4) {
-                v = *reinterpret_cast<const f32x4u*>(p);
-            } else if (left > 0) {
-                v[0] = p[0];
-                if (left > 1) v[1] = p[1];
-                if (left > 2) v[2] = p[2];
-            }
-            r[e] = v;
+            r[e] = distances(graph + i * a.dist_row, j + col, i < a.dist_rows ? limit : 0, false);
         }
     }
     __device__ __forceinline__ void store(float* tile) const {
@@ -323,6 +344,8 @@ __device__ __forceinline__ Bias bias_of(const Args& a, float slope) {
     b.unit = b.plain ? a.scale * kLog2e : kLog2e;
     return b;
 }
+// what is done to every score of a lane's column: n over its tiles, r over a tile's four rows
+#define TRX_EACH_SCORE _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
 template <int N>
 __device__ __forceinline__ bool ordinary(const f32x4 (&d)[N]) {
     uint32_t most = 0;
@@ -331,18 +354,6 @@ __device__ __forceinline__ bool ordinary(const f32x4 (&d)[N]) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) most = max(most, __float_as_uint(d[n][r]));
     return __all(most <= 0x7f800000u);   // neither negative nor NaN
-}
-
-// one column's four distances behind key j: +inf from `limit` on
-__device__ __forceinline__ f32x4 distances(const float* row, int j, int limit, bool whole) {
-    if (whole || j + 4 <= limit) return *reinterpret_cast<const f32x4u*>(row + j);
-    f32x4 d{INFINITY, INFINITY, INFINITY, INFINITY};
-    if (j < limit) {
-        d[0] = row[j];
-        if (j + 1 < limit) d[1] = row[j + 1];
-        if (j + 2 < limit) d[2] = row[j + 2];
-    }
-    return d;
 }
 
 }  // namespace

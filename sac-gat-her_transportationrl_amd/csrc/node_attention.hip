@@ -26,7 +26,7 @@ AttentionCut cut(int64_t kept, int64_t run, int64_t units, int64_t row_bytes, in
     return c;
 }
 int wide_rows(const Args& a) { return a.dtype == 0 && a.channels > 64 ? 64 : 128; }
-int wide_keys(const Args& a) { return a.channels > 64 ? 64 : 128; }
+int wide_bwd(const Args& a) { return a.channels > 64 ? 64 : 128; }
 
 }  // namespace
 
@@ -38,12 +38,12 @@ AttentionCut cut_fwd(const trx_node_attention_args& a) {
 AttentionCut cut_bwd_q(const trx_node_attention_args& a) {
     const int64_t G = a.heads / a.kv_heads;
     return cut(std::min(a.max_queries, a.num_queries) * G, std::min(a.max_nodes, a.num_nodes),
-               (int64_t)a.num_graphs * a.kv_heads, a.num_queries * a.heads * (a.channels + 3) * 4, wide_rows(a), 256);
+               (int64_t)a.num_graphs * a.kv_heads, a.num_queries * a.heads * (a.channels + 3) * 4, wide_bwd(a), 256);
 }
 AttentionCut cut_bwd_kv(const trx_node_attention_args& a) {
     const int64_t G = a.heads / a.kv_heads;
     return cut(std::min(a.max_nodes, a.num_nodes), std::min(a.max_queries, a.num_queries) * G,
-               (int64_t)a.num_graphs * a.kv_heads, a.num_nodes * a.kv_heads * a.channels * 8, wide_keys(a), 256);
+               (int64_t)a.num_graphs * a.kv_heads, a.num_nodes * a.kv_heads * a.channels * 8, wide_bwd(a), 256);
 }
 
 // each row's <go, out> and slope gradient, the slope chunks' sums; the splits of one pass after the other follow

@@ -104,7 +104,10 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
         }
         const float* graph = DIST ? a.dist + b * a.dist_graph : nullptr;
         Distances d_next;
+        int d_row[MQ];
         if (kStageD && first < last) d_next.load(call, graph, tile * kRows, rows, ks.n, first);
+#pragma unroll
+        for (int t = 0; t < MQ; ++t) d_row[t] = min(w * 16 * MQ + 16 * t + c + d_next.shift, kRows - 1) * Distances::kPitch;
         for (int j0 = first; j0 < last; j0 += KT) {
             f32x4 d[MQ][kTiles];
             if (!kAhead) fetch(j0);
@@ -150,40 +153,48 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
                 if (kStageD) {
 #pragma unroll
                     for (int n = 0; n < kTiles; ++n)
-                        d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + (w * 16 * MQ + 16 * t + c) * Distances::kPitch +
-                                                                  16 * n + 4 * g);
+                        d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + d_row[t] + 16 * n + 4 * g);
                 }
-                const bool cut = !DIST && j0 + KT > last, free = DIST && __all(bias[t].slope < 0.0f) && ordinary(d[t]);
                 const float slope = bias[t].slope, unit = bias[t].unit;
-#pragma unroll
-                for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float z = s[t][n][r], slack = 1.0f;
-                        if (CAP) {
-                            const float th = tanh_of<T>(z, bias[t].pre);
-                            z = a.cap * th;
-                            slack = __builtin_fmaf(-th, th, 1.0f);
-                        } else if (!bias[t].plain) {
-                            z = z * bias[t].pre;
-                        }
-                        if (DIST) {
-                            const float y = d[t][n][r];
-                            z = free || finite(y) ? __builtin_fmaf(slope, y, z) : -INFINITY;
-                        } else if (cut && j0 + 16 * n + 4 * g + r >= last) {
-                            z = -INFINITY;
-                        }
-                        const float p = exp2_fast(__builtin_fmaf(z, unit, -lse[t]));
-                        const float v = p * (gp[t][n][r] - D[t]);
-                        if (DIST && slopes) {
-                            // unseen: p and v are zero, and the distance must not be infinite beside them
-                            const float y = free || finite(d[t][n][r]) ? fminf(d[t][n][r], 3e38f) : 0.0f;
-                            sums[t].t += v;
-                            sums[t].pd = __builtin_fmaf(p, y, sums[t].pd);
-                            sums[t].td = __builtin_fmaf(v, y, sums[t].td);
-                        }
-                        u[t][n / 2][4 * (n % 2) + r] = (T)(CAP ? v * slack : v);   // rounded to the type for the product with k
+                f32x4 slack[kTiles];
+                if (CAP) {
+                    TRX_EACH_SCORE {
+                        const float th = tanh_of<T>(s[t][n][r], bias[t].pre);
+                        s[t][n][r] = a.cap * th;
+                        slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
                     }
+                } else if (!bias[t].plain) {
+                    TRX_EACH_SCORE s[t][n][r] *= bias[t].pre;
+                }
+                if (DIST) {
+                    // beside weights of zero a distance must not be infinite in the slopes' sums
+                    if (__all(slope < 0.0f) && ordinary(d[t])) {
+                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope, d[t][n][r], s[t][n][r]);
+                        if (slopes) TRX_EACH_SCORE d[t][n][r] = fminf(d[t][n][r], 3e38f);
+                    } else {
+                        TRX_EACH_SCORE {
+                            const bool seen = finite(d[t][n][r]);
+                            s[t][n][r] = seen ? __builtin_fmaf(slope, d[t][n][r], s[t][n][r]) : -INFINITY;
+                            d[t][n][r] = seen ? d[t][n][r] : 0.0f;
+                        }
+                    }
+                } else if (j0 + KT > last) {
+                    TRX_EACH_SCORE if (j0 + 16 * n + 4 * g + r >= last) s[t][n][r] = -INFINITY;
+                }
+                TRX_EACH_SCORE {
+                    const float p = exp2_fast(__builtin_fmaf(s[t][n][r], unit, -lse[t]));
+                    s[t][n][r] = p;
+                    gp[t][n][r] = p * (gp[t][n][r] - D[t]);
+                }
+                if (DIST && slopes) {
+                    TRX_EACH_SCORE {
+                        sums[t].t += gp[t][n][r];
+                        sums[t].pd = __builtin_fmaf(s[t][n][r], d[t][n][r], sums[t].pd);
+                        sums[t].td = __builtin_fmaf(gp[t][n][r], d[t][n][r], sums[t].td);
+                    }
+                }
+                // rounded to the type for the product with k
+                TRX_EACH_SCORE u[t][n / 2][4 * (n % 2) + r] = (T)(CAP ? gp[t][n][r] * slack[n][r] : gp[t][n][r]);
             }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x)
@@ -329,10 +340,6 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
             __syncthreads();
             if (kAhead && r0 + RT < last) fetch(r0 + RT);
             if (key0 >= ks.n) continue;
-            bool free = falls;
-            if (DIST)
-#pragma unroll
-                for (int t = 0; t < MK; ++t) free = free && ordinary(d[t]);
             f32x4 s[MK][kTiles], gp[MK][kTiles];
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
@@ -352,29 +359,39 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                 }
             }
             frag<T> p[MK][RT / 32], u[MK][RT / 32];
+            f32x4 lse[kTiles], D[kTiles], slope[kTiles];
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(row_lse + 16 * n + 4 * g);
-                const f32x4 D = *reinterpret_cast<const f32x4*>(row_D + 16 * n + 4 * g);
-                const f32x4 slope = DIST ? *reinterpret_cast<const f32x4*>(row_slope + 16 * n + 4 * g) : f32x4{};
+                lse[n] = *reinterpret_cast<const f32x4*>(row_lse + 16 * n + 4 * g);
+                D[n] = *reinterpret_cast<const f32x4*>(row_D + 16 * n + 4 * g);
+                if (DIST) slope[n] = *reinterpret_cast<const f32x4*>(row_slope + 16 * n + 4 * g);
+            }
 #pragma unroll
-                for (int t = 0; t < MK; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float z = s[t][n][r], slack = 1.0f;
-                        if (CAP) {
-                            const float th = tanh_of<T>(z, pre);
-                            z = a.cap * th;
-                            slack = __builtin_fmaf(-th, th, 1.0f);
-                        } else if (!plain) {
-                            z = z * pre;
-                        }
-                        if (DIST) z = free || finite(d[t][n][r]) ? __builtin_fmaf(slope[r], d[t][n][r], z) : -INFINITY;
-                        const float e = exp2_fast(__builtin_fmaf(z, unit, -lse[r]));
-                        const float v = e * (gp[t][n][r] - D[r]), x = CAP ? v * slack : v;
-                        p[t][n / 2][4 * (n % 2) + r] = (T)e;   // both rounded to the type for their products
-                        u[t][n / 2][4 * (n % 2) + r] = (T)x;
+            for (int t = 0; t < MK; ++t) {
+                f32x4 slack[kTiles];
+                if (CAP) {
+                    TRX_EACH_SCORE {
+                        const float th = tanh_of<T>(s[t][n][r], pre);
+                        s[t][n][r] = a.cap * th;
+                        slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
                     }
+                } else if (!plain) {
+                    TRX_EACH_SCORE s[t][n][r] *= pre;
+                }
+                if (DIST) {
+                    if (falls && ordinary(d[t])) {
+                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope[n][r], d[t][n][r], s[t][n][r]);
+                    } else {
+                        TRX_EACH_SCORE s[t][n][r] =
+                            finite(d[t][n][r]) ? __builtin_fmaf(slope[n][r], d[t][n][r], s[t][n][r]) : -INFINITY;
+                    }
+                }
+                TRX_EACH_SCORE {   // both rounded to the type for their products
+                    const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, -lse[n][r]));
+                    const float v = e * (gp[t][n][r] - D[n][r]);
+                    p[t][n / 2][4 * (n % 2) + r] = (T)e;
+                    u[t][n / 2][4 * (n % 2) + r] = (T)(CAP ? v * slack[n][r] : v);
+                }
             }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x)
@@ -486,7 +503,8 @@ void launch_bwd(const Args& a, hipStream_t stream) {
     float *chunks = slopes + a.num_queries * a.heads, *split = dots + attention_row_floats(a);
     const bool want_slopes = DIST && a.grad_slope && a.slope;
     auto blocks = [](int64_t n) { return (unsigned)std::min<int64_t>(2048, (n / 4 + 255) / 256); };
-    constexpr int M = kTilesOfWave<T, CP>, MK = CP == 128 ? 1 : 2;
+    // 128 channels: of 32 rows a wave, operands, accumulators and both score tiles leave no registers to load ahead
+    constexpr int M = kTilesOfWave<T, CP>, MQ = CP == 128 ? 1 : 2, MK = CP == 128 ? 1 : 2;
     if (a.num_queries > 0) {
         const AttentionCut c = cut_bwd_q(a);
         float* part = c.splits > 1 ? split : nullptr;
@@ -496,7 +514,7 @@ void launch_bwd(const Args& a, hipStream_t stream) {
             hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, M, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
                                want_slopes ? slopes : nullptr, part);
         else
-            hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, M, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call, dots,
+            hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, MQ, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call, dots,
                                want_slopes ? slopes : nullptr, part);
         const int64_t n = a.num_queries * a.heads * a.channels;
         if (part)

@@ -77,7 +77,10 @@ attention_fwd_kernel(Call call, float* part) {
         }
         const float* graph = DIST ? a.dist + b * a.dist_graph : nullptr;
         Distances d_next;
+        int d_row[MQ];
         if (kStageD && first < last) d_next.load(call, graph, tile * kRows, rows, ks.n, first);
+#pragma unroll
+        for (int t = 0; t < MQ; ++t) d_row[t] = min(w * 16 * MQ + 16 * t + c + d_next.shift, kRows - 1) * Distances::kPitch;
         for (int j0 = first; j0 < last; j0 += KT) {
             f32x4 d[MQ][kTiles];
             if (!kAhead) fetch(j0);
@@ -117,30 +120,27 @@ attention_fwd_kernel(Call call, float* part) {
                 if (kStageD) {
 #pragma unroll
                     for (int n = 0; n < kTiles; ++n)
-                        d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + (w * 16 * MQ + 16 * t + c) * Distances::kPitch +
-                                                                  16 * n + 4 * g);
+                        d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + d_row[t] + 16 * n + 4 * g);
                 }
                 // scores in bias.unit, and their maximum
-#define EACH_SCORE                  \
-    _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
                 if (CAP) {
-                    EACH_SCORE s[t][n][r] = a.cap * tanh_of<T>(s[t][n][r], bias[t].pre);
+                    TRX_EACH_SCORE s[t][n][r] = a.cap * tanh_of<T>(s[t][n][r], bias[t].pre);
                 } else if (!bias[t].plain) {
-                    EACH_SCORE s[t][n][r] *= bias[t].pre;
+                    TRX_EACH_SCORE s[t][n][r] *= bias[t].pre;
                 }
                 if (DIST) {
                     const float slope = bias[t].slope;
                     if (__all(slope < 0.0f) && ordinary(d[t])) {
-                        EACH_SCORE s[t][n][r] = __builtin_fmaf(slope, d[t][n][r], s[t][n][r]);
+                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope, d[t][n][r], s[t][n][r]);
                     } else {
-                        EACH_SCORE s[t][n][r] =
+                        TRX_EACH_SCORE s[t][n][r] =
                             finite(d[t][n][r]) ? __builtin_fmaf(slope, d[t][n][r], s[t][n][r]) : -INFINITY;
                     }
                 } else if (j0 + KT > last) {
-                    EACH_SCORE if (j0 + 16 * n + 4 * g + r >= last) s[t][n][r] = -INFINITY;
+                    TRX_EACH_SCORE if (j0 + 16 * n + 4 * g + r >= last) s[t][n][r] = -INFINITY;
                 }
                 float top = -INFINITY;
-                EACH_SCORE top = fmaxf(top, s[t][n][r]);
+                TRX_EACH_SCORE top = fmaxf(top, s[t][n][r]);
                 top = column_max(top) * bias[t].unit;
                 // The reference point moves only when a score passes it by 2^8: nothing is lost in float32, and the
                 // accumulators are rescaled once or twice a row instead of at every new maximum.
@@ -153,12 +153,11 @@ attention_fwd_kernel(Call call, float* part) {
                     for (int x = 0; x < CP / 16; ++x) o[t][x] = o[t][x] * f;
                 }
                 const float base = m[t] == -INFINITY ? 0.0f : -m[t], unit = bias[t].unit;
-                EACH_SCORE {
+                TRX_EACH_SCORE {
                     const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, base));
                     l[t] += e;
                     p[t][n / 2][4 * (n % 2) + r] = (T)e;   // rounded to the type for the product with v
                 }
-#undef EACH_SCORE
             }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x)
