@@ -884,7 +884,8 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
  * max_queries / max_nodes: the largest graph's rows; they only shape the
  * launch (a smaller value costs time, never rows).  Sums and the softmax's
  * statistics are float32; probabilities and score gradients enter the matrix
- * products in dtype.  Deterministic: no float atomics.  workspace:
+ * products in dtype.  Deterministic: no float atomics.  At most 2^23 / heads
+ * graphs.  workspace:
  * trx_node_attention_workspace_bytes(args, backward) bytes, 16-byte aligned
  * (0: may be NULL).                                                        */
 #define TRX_ATT_MAX_CHANNELS 128
@@ -931,7 +932,7 @@ int trx_node_attention_backward(const trx_node_attention_args* a, void* stream);
  * entropy) + sum_t g_top[t] (1[j = top_action[t]] - p_j); 0 where a link may
  * not be chosen, and for packed elements of no row; an action of log_prob -inf
  * passes nothing.  The g_* may be NULL.  max_row: the longest packed row; it
- * only shapes the launch.  workspace: trx_action_log_probs_workspace_bytes
+ * only shapes the launch.  At most 2^23 rows, 2^30 links in one.  workspace: trx_action_log_probs_workspace_bytes
  * bytes, 16-byte aligned (0: may be NULL; the forward's only).             */
 #define TRX_TOP_MAX 16
 typedef struct trx_action_log_probs_args {

@@ -1351,6 +1351,8 @@ int check_attention(const trx_node_attention_args* a, bool backward) {
     if (rc) return rc;
     if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0.0f)
         return fail(TRX_EINVAL, "node_attention: scale must be finite and cap finite and >= 0");
+    if (a->cap > 0.0f && !(std::fabs(a->scale / a->cap) < 1e30f))
+        return fail(TRX_EINVAL, "node_attention: cap %g is too small beside scale %g", (double)a->cap, (double)a->scale);
     if (!a->q_ptr || !a->k_ptr) return fail(TRX_EINVAL, "node_attention: NULL q_ptr / k_ptr");
     if (a->num_queries > 0 && (!a->q || !a->out)) return fail(TRX_EINVAL, "node_attention: NULL q / out");
     if (a->num_nodes > 0 && (!a->k || !a->v)) return fail(TRX_EINVAL, "node_attention: NULL k / v");
@@ -1379,7 +1381,7 @@ int check_log_probs_shape(const trx_action_log_probs_args* a) {
     if (!a) return fail(TRX_EINVAL, "action_log_probs: args is NULL");
     if (a->rows < 0 || a->row_len < 0 || a->row_stride < 0 || a->total < 0 || a->max_row < 0 || a->mask_stride < 0)
         return fail(TRX_EINVAL, "action_log_probs: negative size");
-    if (a->rows > (int64_t(1) << 31) - 1) return fail(TRX_EUNSUP, "action_log_probs: at most 2^31 - 1 rows");
+    if (a->rows > (1 << 23)) return fail(TRX_EUNSUP, "action_log_probs: at most 2^23 rows");
     if (a->row_len > (int64_t(1) << 30) || a->max_row > (int64_t(1) << 30))
         return fail(TRX_EUNSUP, "action_log_probs: at most 2^30 links in a row");
     if (a->dtype < 0 || a->dtype > 2 || a->mask_dtype < 0 || a->mask_dtype > 1)

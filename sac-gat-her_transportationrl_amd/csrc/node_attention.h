@@ -302,17 +302,6 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh(x * mul): for two-byte types 1 - 2 / (1 + e^2x) with the hardware's exp2
-// and reciprocal, off by about 2^-23 absolute, far below their products' own
-// rounding; float32 takes the library's
-template <typename T>
-__device__ __forceinline__ float tanh_of(float x, float mul) {
-    if constexpr (sizeof(T) == 2)
-        return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + exp2_fast(x * (mul * 2.0f * kLog2e))), 1.0f);
-    else
-        return tanhf(x * mul);
-}
-
 // sums and maxima over the four lanes that share a column (same c)
 __device__ __forceinline__ float column_sum(float v) {
     v += __shfl_xor(v, 16);
@@ -346,6 +335,44 @@ __device__ __forceinline__ Bias bias_of(const Args& a, float slope) {
 }
 // what is done to every score of a lane's column: n over its tiles, r over a tile's four rows
 #define TRX_EACH_SCORE _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
+// Scores capped: cap tanh(s * pre), and with SLACK the tanh's slope 1 - tanh^2.  float32 takes the library's tanh.  For
+// two-byte types: 1 - 2 / (1 + e^2x) by the hardware's exp2 and reciprocal, off by about 2^-23, so within a quarter of
+// zero, where that is too much beside x (and all of it for a large cap), the series to x^7, off by 4e-7 of x there.  A
+// tile whose arguments all lie there needs nothing else, which is the common case and the cheap one.
+template <typename T, int kTiles, bool SLACK>
+__device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles], float pre, float cap) {
+    if constexpr (sizeof(T) == 4) {
+        TRX_EACH_SCORE {
+            const float th = tanhf(s[n][r] * pre);
+            s[n][r] = cap * th;
+            if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
+        }
+    } else {
+        float most = 0.0f;
+        TRX_EACH_SCORE {
+            s[n][r] *= pre;
+            most = fmaxf(most, fabsf(s[n][r]));
+        }
+        auto series = [](float x) {
+            const float y = x * x;
+            return x * __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+        };
+        if (__all(most < 0.25f)) {
+            TRX_EACH_SCORE {
+                const float th = series(s[n][r]);
+                s[n][r] = cap * th;
+                if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
+            }
+        } else {
+            TRX_EACH_SCORE {
+                const float x = s[n][r], e = exp2_fast(x * (2.0f * kLog2e));
+                const float th = fabsf(x) < 0.25f ? series(x) : __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+                s[n][r] = cap * th;
+                if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
+            }
+        }
+    }
+}
 template <int N>
 __device__ __forceinline__ bool ordinary(const f32x4 (&d)[N]) {
     uint32_t most = 0;

@@ -158,11 +158,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
                 const float slope = bias[t].slope, unit = bias[t].unit;
                 f32x4 slack[kTiles];
                 if (CAP) {
-                    TRX_EACH_SCORE {
-                        const float th = tanh_of<T>(s[t][n][r], bias[t].pre);
-                        s[t][n][r] = a.cap * th;
-                        slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
-                    }
+                    cap_scores<T, kTiles, true>(s[t], slack, bias[t].pre, a.cap);
                 } else if (!bias[t].plain) {
                     TRX_EACH_SCORE s[t][n][r] *= bias[t].pre;
                 }
@@ -370,11 +366,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
             for (int t = 0; t < MK; ++t) {
                 f32x4 slack[kTiles];
                 if (CAP) {
-                    TRX_EACH_SCORE {
-                        const float th = tanh_of<T>(s[t][n][r], pre);
-                        s[t][n][r] = a.cap * th;
-                        slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
-                    }
+                    cap_scores<T, kTiles, true>(s[t], slack, pre, a.cap);
                 } else if (!plain) {
                     TRX_EACH_SCORE s[t][n][r] *= pre;
                 }

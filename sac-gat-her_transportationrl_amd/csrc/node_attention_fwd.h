@@ -124,7 +124,7 @@ attention_fwd_kernel(Call call, float* part) {
                 }
                 // scores in bias.unit, and their maximum
                 if (CAP) {
-                    TRX_EACH_SCORE s[t][n][r] = a.cap * tanh_of<T>(s[t][n][r], bias[t].pre);
+                    cap_scores<T, kTiles, false>(s[t], s[t], bias[t].pre, a.cap);
                 } else if (!bias[t].plain) {
                     TRX_EACH_SCORE s[t][n][r] *= bias[t].pre;
                 }

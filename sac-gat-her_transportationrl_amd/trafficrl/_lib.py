@@ -495,17 +495,6 @@ def raw_stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def once(backward):
-    """once_differentiable without its cost where no second derivative is asked for."""
-    import torch
-    from torch.autograd.function import once_differentiable
-    guarded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
-
-
 def stream_ptr(device=None) -> ctypes.c_void_p:
     import torch
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)

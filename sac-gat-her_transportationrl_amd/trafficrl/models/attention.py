@@ -9,6 +9,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
+from ..autograd import once
 
 
 def _strided(t: torch.Tensor) -> torch.Tensor:
@@ -32,7 +33,8 @@ def _args(q, k, v, ptr, k_ptr, dist, slope, rest, out, low, lse, backward: bool,
     v_row, v_head, _ = v.stride()
     d = (0, 0, 0, 0, 0, 0)
     if dist is not None:
-        d = (*dist.shape[-2:], dist.data_ptr(), dist.stride(0) if dist.dim() == 3 else 0, dist.stride(-2),
+        # an empty matrix shows no pair, which a null pointer would not say
+        d = (*dist.shape[-2:], dist.data_ptr() or ptr.data_ptr(), dist.stride(0) if dist.dim() == 3 else 0, dist.stride(-2),
              0 if slope is None else slope.data_ptr())
     a = _lib.TrxNodeAttentionArgs(
         ptr.numel() - 1, heads, kv_heads, channels, code, d[0], d[1], scale, cap, max_queries, max_nodes, rows, nodes,
@@ -79,7 +81,7 @@ class _NodeAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @_lib.once
+    @once("node_attention")
     def backward(ctx, grad_out):
         return *_lib.on_device(grad_out.device, _launch_backward, *ctx.saved_tensors, ctx.rest, grad_out,
                                ctx.needs_input_grad[3]), None, None, None, None
@@ -153,6 +155,8 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
     cap = float(cap)
     if not math.isfinite(scale) or not math.isfinite(cap) or cap < 0.0:
         raise ValueError(f"{what}: scale must be finite, cap finite and >= 0 (got {scale}, {cap})")
+    if cap > 0.0 and not abs(scale) < cap * 1e30:
+        raise ValueError(f"{what}: cap {cap} is too small beside scale {scale}")
     max_queries = q.shape[0] if max_queries is None else int(max_queries)
     max_nodes = k.shape[0] if max_nodes is None else int(max_nodes)
     if max_queries < 0 or max_nodes < 0:

@@ -9,6 +9,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
+from ..autograd import once
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -46,7 +47,7 @@ class _DropoutAdd(torch.autograd.Function):
         return y
 
     @staticmethod
-    @_lib.once
+    @once("dropout_add")
     def backward(ctx, grad_y):
         wants_x, wants_residual = ctx.needs_input_grad[:2]
         grad_x = None

@@ -8,6 +8,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
+from ..autograd import once
 
 
 _MASK_TYPES = (torch.float32, torch.bool, torch.uint8)
@@ -70,7 +71,7 @@ class _ActionLogProbs(torch.autograd.Function):
         return tuple(outs)
 
     @staticmethod
-    @_lib.once
+    @once("action_log_probs")
     def backward(ctx, *grads):
         logits = ctx.saved_tensors[0]
         return _lib.on_device(logits.device, _launch_backward, *ctx.saved_tensors, ctx.rest,

@@ -82,7 +82,7 @@ def test_shared_heads(H, Hk, dt):
     check([24, 90, 3], H, Hk, 32, dt, "shared", queries=[1, 5, 2])
 
 
-@pytest.mark.parametrize("cap", [0.5, 10.0, 50.0])
+@pytest.mark.parametrize("cap", [0.5, 10.0, 50.0, 1e4])
 @pytest.mark.parametrize("dt", [F32, BF16, F16], ids=str)
 def test_cap(cap, dt):
     check([24, 100], 4, 2, 64, dt, "each", cap=cap)
@@ -188,6 +188,45 @@ def test_extreme_scores():
     out = node_attention(q, k, v, ints(p), dist=dist, slope=torch.full((2,), 3e38, device="cuda"))
     # the one key left has some weight p, and out = fl(fl(p v) fl(1 / p)): three roundings, under 4 u |v|
     assert_within("out", out, v.double(), 4 * 2.0 ** -24 * v.double().abs())
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=str)
+def test_scale_and_slope_signs(dt):
+    """A scale of zero, negative and tiny ones; slopes of zero, negative and mixed ones."""
+    from trafficrl.models import node_attention
+    for sizes in ([30, 24], [150, 70]):
+        q, k, v, p, _, dist, _, go = make(sizes, 4, 2, 32, dt, "shared")
+        for scale in (0.0, -0.2, 1e-25, 0.3):
+            for slope in ([0.0] * 4, [-0.5] * 4, [0.5, -0.25, 0.0, 1.0], [1.0] * 4):
+                s = torch.tensor(slope, device="cuda").requires_grad_()
+                leaves = [t.detach().requires_grad_() for t in (q, k, v)] + [s]
+                out = node_attention(*leaves[:3], ints(p), dist=dist, slope=s, scale=scale)
+                want = reference(q, k, v, p, p, dist, s.detach(), scale, 0.0, go)
+                assert_within("out", out, *want["out"])
+                for name, t in zip(["q", "k", "v", "slope"], torch.autograd.grad(out, leaves, go)):
+                    assert_within(name, t, *want[name])
+
+
+def test_large_cap_is_no_cap():
+    """cap = 1e6: a capped score differs from the plain one by z^3 / 3e12, below float32's resolution of z here, so the
+    half types' fast tanh must not show."""
+    from trafficrl.models import node_attention
+    for dt in (F32, BF16, F16):
+        q, k, v, p, _, dist, slope, _ = make([40, 200], 4, 2, 64, dt, "shared")
+        out = node_attention(q, k, v, ints(p), dist=dist, slope=slope, cap=1e6)
+        assert_within("out", out, *reference(q, k, v, p, p, dist, slope)["out"])
+
+
+def test_pointers_outside_the_tensors():
+    """ptr values past the rows, or negative, are clamped; an empty distance matrix shows no pair."""
+    from trafficrl.models import node_attention
+    q, k, v, _, _, _, _, _ = make([40, 30], 2, 2, 32, F32)
+    a = node_attention(q, k, v, ints([-5, 40, 10 ** 12]))
+    assert torch.equal(a, node_attention(q, k, v, ints([0, 40, 70])))
+    a = node_attention(q, k, v, ints([10 ** 12, 10 ** 12 + 1]))
+    assert bool((a == 0).all())
+    for shape in ((0, 0), (40, 0), (0, 40)):
+        assert bool((node_attention(q, k, v, ints([0, 40, 70]), dist=torch.zeros(shape, device="cuda")) == 0).all())
 
 
 def test_no_rows():

@@ -45,7 +45,7 @@ P = torch.tensor([0, 2, 6])
     dict(dist=torch.zeros(6, 6, dtype=torch.float64)), dict(dist=torch.zeros(3, 6, 6)), dict(dist=torch.zeros(36)),
     dict(dist=torch.zeros(6, 6, requires_grad=True)), dict(slope=torch.zeros(4)),
     dict(dist=torch.zeros(6, 6), slope=torch.zeros(3)), dict(dist=torch.zeros(6, 6), slope=torch.zeros(4).double()),
-    dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.inf), dict(max_nodes=-1),
+    dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.inf), dict(cap=1e-35), dict(max_nodes=-1),
 ], ids=lambda c: ",".join(c))
 def test_node_attention_refuses(change):
     from trafficrl.models import node_attention
@@ -116,7 +116,7 @@ def _attention_args():
 @pytest.mark.parametrize("field,value,code", [
     ("num_graphs", -1, -1), ("num_queries", -1, -1), ("num_nodes", 1 << 31, -3), ("dtype", 3, -1), ("kv_heads", 3, -1),
     ("kv_heads", 0, -1), ("heads", 2048, -3), ("channels", 33, -3), ("channels", 136, -3), ("channels", 0, -3),
-    ("scale", math.nan, -1), ("cap", -1.0, -1), ("q", None, -1), ("v", None, -1), ("q_ptr", None, -1),
+    ("scale", math.nan, -1), ("cap", -1.0, -1), ("cap", 1e-35, -1), ("q", None, -1), ("v", None, -1), ("q_ptr", None, -1),
     ("k_ptr", None, -1), ("out", None, -1), ("q", 4100, -1), ("k_row", 65, -1), ("v_head", -32, -1),
     ("lse", None, -1), ("grad_out", None, -1), ("grad_k", None, -1), ("grad_v", 4104, -1),
     ("workspace", None, -1), ("workspace_bytes", 4, -1), ("workspace", 4100, -1)])
@@ -150,7 +150,7 @@ def _log_probs_args():
 
 
 @pytest.mark.parametrize("field,value,code", [
-    ("rows", -1, -1), ("rows", 1 << 31, -3), ("row_len", -1, -1), ("row_len", 1 << 31, -3), ("dtype", 3, -1),
+    ("rows", -1, -1), ("rows", (1 << 23) + 1, -3), ("row_len", -1, -1), ("row_len", 1 << 31, -3), ("dtype", 3, -1),
     ("mask_dtype", 2, -1), ("top_k", 17, -3), ("top_k", -1, -3), ("logits", None, -1), ("action", None, -1),
     ("stats", None, -1), ("log_prob", None, -1), ("top_action", None, -1), ("top_log_prob", None, -1)])
 def test_log_probs_boundary(field, value, code):

@@ -113,3 +113,20 @@ def test_agent_evaluates_actions(grad):
         got = torch.autograd.grad(r.log_prob.sum() - r.entropy.sum(), params, allow_unused=True)
         assert any(t is not None and bool(t.abs().max() > 0) for t in got)
         assert all(t is None or bool(torch.isfinite(t).all()) for t in got)
+
+
+def test_second_derivatives_are_refused():
+    """create_graph works, but what comes back is no constant: differentiating it
+    raises, also where the incoming gradient does not require one."""
+    from trafficrl.models import dropout_add, node_attention
+    from trafficrl.rl import action_log_probs
+    rng, p = torch.tensor([1, 2], device="cuda"), torch.tensor([0, 10], device="cuda")
+    x = torch.randn(10, 2, 32, device="cuda", requires_grad=True)
+    logits = torch.randn(4, 9, device="cuda", requires_grad=True)
+    for y, leaf in ((node_attention(x, x, x, p), x), (dropout_add(x, rng, 0.5, residual=x), x),
+                    (action_log_probs(logits, torch.zeros(4, dtype=torch.int64, device="cuda")).log_prob, logits)):
+        g, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+        want, = torch.autograd.grad(y.sum(), leaf, retain_graph=True)
+        assert torch.equal(g, want)
+        with pytest.raises(RuntimeError, match="once, not twice"):
+            ((g * g).sum() + leaf.sum()).backward()
