@@ -247,9 +247,11 @@ __device__ __forceinline__ void put4(T* out, T* low, int64_t at, f32x4 v) {
 template <typename T, int CP>
 constexpr int kTilesOfWave = sizeof(T) == 4 && CP == 128 ? 1 : 2;
 
-// waves of a SIMD that registers are left for
+// Waves of a SIMD that registers are left for.  For a workgroup of one wave the compiler's own choice takes accumulator
+// registers beside the others and so fits fewer: 4096 networks of 24 nodes, 4 heads of 64, forward, 42 us with 2 asked
+// for, 50 us without, 66 us with 4 (spills).
 template <typename T, int CP, int WAVES>
-constexpr int kWavesPerSimd = WAVES > 1 ? 2 : 1;
+constexpr int kWavesPerSimd = WAVES > 1 || CP <= 64 ? 2 : 1;
 
 // calls f with the padded channels, whether there are distances, whether scores are capped
 template <typename T, typename F>
@@ -336,9 +338,10 @@ __device__ __forceinline__ Bias bias_of(const Args& a, float slope) {
 // what is done to every score of a lane's column: n over its tiles, r over a tile's four rows
 #define TRX_EACH_SCORE _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
 // Scores capped: cap tanh(s * pre), and with SLACK the tanh's slope 1 - tanh^2.  float32 takes the library's tanh.  For
-// two-byte types: 1 - 2 / (1 + e^2x) by the hardware's exp2 and reciprocal, off by about 2^-23, so within a quarter of
-// zero, where that is too much beside x (and all of it for a large cap), the series to x^7, off by 4e-7 of x there.  A
-// tile whose arguments all lie there needs nothing else, which is the common case and the cheap one.
+// two-byte types, a tile whose arguments all lie within a quarter of zero takes the series to x^7 (off by 4e-7 of x at
+// the end), seven operations; others 1 - 2 / (1 + e^2x) by the hardware's exp2 and reciprocal, twelve, off by 2^-23:
+// 8e-6 in a score at a cap of 64, far below what rounding its probability takes.  With larger caps that error would
+// grow past the scores' own, so there arguments within a quarter of zero take the series wherever they are.
 template <typename T, int kTiles, bool SLACK>
 __device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles], float pre, float cap) {
     if constexpr (sizeof(T) == 4) {
@@ -360,6 +363,13 @@ __device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kT
         if (__all(most < 0.25f)) {
             TRX_EACH_SCORE {
                 const float th = series(s[n][r]);
+                s[n][r] = cap * th;
+                if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
+            }
+        } else if (cap <= 64.0f) {
+            TRX_EACH_SCORE {
+                const float e = exp2_fast(s[n][r] * (2.0f * kLog2e));
+                const float th = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
                 s[n][r] = cap * th;
                 if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
             }

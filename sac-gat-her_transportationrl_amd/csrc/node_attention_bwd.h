@@ -514,7 +514,7 @@ void launch_bwd(const Args& a, hipStream_t stream) {
                                SplitSum{part, a.grad_q, a.scale}, SplitSum{}, c.splits, n, n,
                                (int64_t)a.heads * a.channels, a.q_ptr, a.num_graphs, a.num_queries);
         if (want_slopes) {
-            const int count = (int)std::max<int64_t>(1, std::min<int64_t>(kSlopeChunks, a.num_queries / 2048));
+            const int count = (int)std::max<int64_t>(1, std::min<int64_t>(kSlopeChunks, a.num_queries / 16384));
             hipLaunchKernelGGL(slope_rows_kernel<T>, dim3(a.heads, count), dim3(1024), 0, stream, a, slopes,
                                part ? part + c.splits * n : nullptr, c.splits, count > 1 ? chunks : a.grad_slope);
             if (count > 1)

@@ -125,18 +125,19 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
     code = _lib.float_code(q, f"{what}: q")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{what}: q, k, v differ in type: {q.dtype}, {k.dtype}, {v.dtype}")
-    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+    rows, H, C = q.shape
+    nodes, kv_heads, channels = k.shape
+    if k.shape != v.shape or channels != C:
         raise ValueError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit together")
-    H, C = q.shape[1], q.shape[2]
-    if H < 1 or k.shape[1] < 1 or H % k.shape[1]:
-        raise ValueError(f"{what}: {k.shape[1]} key/value heads must divide {H} heads")
+    if H < 1 or kv_heads < 1 or H % kv_heads:
+        raise ValueError(f"{what}: {kv_heads} key/value heads must divide {H} heads")
     if C < 8 or C % 8 or C > _lib.ATT_MAX_CHANNELS:
         raise ValueError(f"{what}: channels must be a multiple of 8 up to {_lib.ATT_MAX_CHANNELS}, got {C}")
     if k_ptr is None:
-        if q.shape[0] != k.shape[0]:
-            raise ValueError(f"{what}: {q.shape[0]} query rows and {k.shape[0]} nodes need a k_ptr")
+        if rows != nodes:
+            raise ValueError(f"{what}: {rows} query rows and {nodes} nodes need a k_ptr")
         k_ptr = ptr
-    for p in (ptr, k_ptr):
+    for p in (ptr,) if k_ptr is ptr else (ptr, k_ptr):
         if p.dtype != torch.int64 or p.dim() != 1 or p.numel() != ptr.numel() or p.numel() < 1:
             raise ValueError(f"{what}: ptr and k_ptr must be int64 [networks + 1]")
     if dist is not None:
@@ -157,8 +158,8 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
         raise ValueError(f"{what}: scale must be finite, cap finite and >= 0 (got {scale}, {cap})")
     if cap > 0.0 and not abs(scale) < cap * 1e30:
         raise ValueError(f"{what}: cap {cap} is too small beside scale {scale}")
-    max_queries = q.shape[0] if max_queries is None else int(max_queries)
-    max_nodes = k.shape[0] if max_nodes is None else int(max_nodes)
+    max_queries = rows if max_queries is None else int(max_queries)
+    max_nodes = nodes if max_nodes is None else int(max_nodes)
     if max_queries < 0 or max_nodes < 0:
         raise ValueError(f"{what}: max_queries and max_nodes must be >= 0")
     _lib.same_device(what, q, k, v, ptr, k_ptr, dist, slope)
