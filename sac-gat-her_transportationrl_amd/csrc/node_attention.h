@@ -22,6 +22,15 @@
 #include "trx_internal.h"
 
 namespace trx {
+
+// How a pass over kept rows (tiles of them) and an axis that is run over (splits of it) is cut
+struct AttentionCut {
+    bool narrow;   // one wave
+    int mq;        // its 16-row tiles
+    int64_t tiles;
+    int splits;
+};
+
 namespace {
 
 constexpr int kWave = 64;
@@ -141,22 +150,23 @@ inline Divide divide_by(int d) {
     return {(uint32_t)((uint64_t(1) << (31 + s)) / d + 1), 31 + s, (uint32_t)d};
 }
 
-// The arguments of a launch.  grid.x: every (tile, graph, key/value head) in this order, so that the tiles of one
-// (graph, head), which read the same keys, lie 8 k blocks apart where there are 8 k heads: on one die, behind one
-// L2.  Then kRestBlocks workgroups for the rows of no graph; they must not lie between the others, or every second
-// compute unit gets nothing else.  grid.z: the splits.
-// Where there are distances, each die gets consecutive (tile, graph, head)s instead: the heads of a tile read the
-// same distances, 4 bytes a pair and head that would otherwise come through the fabric once a die.
+// The arguments of a launch.  The grid: every (tile, split, graph, key/value head) in this order, last tiles first:
+// only large graphs have them, and their workgroups, the longest, had better not start last.  Behind them kRestBlocks
+// workgroups for the rows of no graph; they must not lie between the others, or every second compute unit gets nothing
+// else.  Eight dies take workgroups in turn, so the tiles of one (graph, head), which read the same keys, lie behind one
+// L2 where there are 8 k heads.  Where there are distances, the heads of a tile go to one die instead: they read the
+// same 4 bytes a pair and head, which would otherwise come through the fabric once a die.
 constexpr int kRestBlocks = 16;
 struct Call {
     Args a;
     Divide group, kv, units;   // by heads of a group, key/value heads, (graph, key/value head)s
+    Divide splits;
     int tiles, blocks;
 };
-inline Call call_of(const Args& a, int64_t tiles) {
+inline Call call_of(const Args& a, const AttentionCut& c) {
     const int units = a.num_graphs * a.kv_heads;
-    return {a, divide_by(a.heads / a.kv_heads), divide_by(a.kv_heads), divide_by(units > 0 ? units : 1), (int)tiles,
-            (int)tiles * units};
+    return {a, divide_by(a.heads / a.kv_heads), divide_by(a.kv_heads), divide_by(units > 0 ? units : 1),
+            divide_by(c.splits), (int)c.tiles, (int)c.tiles * c.splits * units};
 }
 
 // one column's four distances behind key j: +inf from `limit` on
@@ -266,10 +276,21 @@ inline hipError_t by_shape(const Args& a, F&& f) {
     return second(std::integral_constant<int, 128>{});
 }
 
+// what a workgroup does
+struct Work {
+    int tile, split, graph, head;   // key/value head
+};
 template <bool DIST>
-__device__ __forceinline__ int work_of(const Call& call) {
-    const int id = blockIdx.x, each = call.blocks / 8;   // 8 dies take workgroups in turn
-    return DIST && id < 8 * each ? id % 8 * each + id / 8 : id;
+__device__ __forceinline__ Work work_of(const Call& call) {
+    int id = blockIdx.x;
+    const int heads = call.a.kv_heads, groups = call.kv(call.blocks) & ~7;
+    if (DIST && id < groups * heads) {
+        // eight graphs' worth at a time, turned from lot to lot, or a graph would always meet the same die
+        const int slot = id >> 3, lot = call.kv(slot), turn = lot + (lot >> 3) + (lot >> 6);
+        id = (lot * 8 + ((id + turn) & 7)) * heads + (slot - lot * heads);
+    }
+    const int of = call.units(id), unit = id - of * call.units.by, tile = call.splits(of), graph = call.kv(unit);
+    return {call.tiles - 1 - tile, of - tile * (int)call.splits.by, graph, unit - graph * heads};
 }
 
 struct Span {
@@ -395,14 +416,6 @@ __device__ __forceinline__ bool ordinary(const f32x4 (&d)[N]) {
 
 }  // namespace
 
-// How a pass over kept rows (grid.y tiles of them) and an axis that is run over
-// (grid.z splits of it) is cut
-struct AttentionCut {
-    bool narrow;   // one wave
-    int mq;        // its 16-row tiles
-    int64_t tiles;
-    int splits;
-};
 // node_attention_fwd.h, node_attention_bwd.h; instantiated in node_attention_{f32,bf16,f16}.hip
 template <typename T>
 hipError_t launch_attention_fwd(const trx_node_attention_args& a, hipStream_t stream);

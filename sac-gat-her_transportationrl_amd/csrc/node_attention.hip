@@ -22,11 +22,12 @@ AttentionCut cut(int64_t kept, int64_t run, int64_t all, int64_t graphs, int64_t
     c.narrow = kept <= 32;
     c.mq = c.narrow && kept <= 16 ? 1 : 2;
     const int64_t each = c.narrow ? 16 * c.mq : wide;
-    c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, (1 << 23) / units));   // grid.x x 256 < 2^32
+    c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, (1 << 23) / units));
     const int64_t blocks = std::max<int64_t>(1, std::min(units * c.tiles, heads * (all / each + graphs)));
     const int64_t want = c.narrow ? 2048 : 512;
     const int64_t most = std::min<int64_t>(64, std::min(run / least, (int64_t(1) << 28) / std::max<int64_t>(1, row_bytes)));
     c.splits = (int)std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, most));
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(c.splits, (1 << 23) / (units * c.tiles)));   // the grid x 256 < 2^32
     return c;
 }
 int wide_rows(const Args& a) { return a.dtype == 0 && a.channels > 64 ? 64 : 128; }

@@ -38,20 +38,20 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
         if (!part) zero_rest(grad_q, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
         return;
     }
-    const int tile0 = call.units(work_of<DIST>(call)), of = work_of<DIST>(call) - tile0 * call.units.by;
-    const int b = call.kv(of), hk = of - b * a.kv_heads;
+    const Work work = work_of<DIST>(call);
+    const int b = work.graph, hk = work.head, split = work.split, splits = call.splits.by;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
     int first = 0, last = ks.n;
-    if (gridDim.z > 1) {
-        const int each = ((ks.n + KT - 1) / KT + gridDim.z - 1) / gridDim.z * KT;
-        first = min((int64_t)ks.n, (int64_t)blockIdx.z * each);
+    if (splits > 1) {
+        const int each = ((ks.n + KT - 1) / KT + splits - 1) / splits * KT;
+        first = min((int64_t)ks.n, (int64_t)split * each);
         last = min(ks.n, first + each);
     }
     const T* k_base = static_cast<const T*>(a.k) + ks.at * a.k_row + hk * a.k_head;
     const T* v_base = static_cast<const T*>(a.v) + ks.at * a.v_row + hk * a.v_head;
 
-    for (int tile = tile0; (int64_t)tile * kRows < rows; tile += call.tiles) {
+    for (int tile = work.tile; (int64_t)tile * kRows < rows; tile += call.tiles) {
         const int row0 = tile * kRows + w * 16 * MQ;
         Staged<T, CP, KT, kThreads> k_next, v_next;
         auto fetch = [&](int j0) {
@@ -97,7 +97,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
             }
             lse[t] = a.lse[at];
             if (lse[t] == -INFINITY) lse[t] = INFINITY;   // an empty row: every probability comes out as zero
-            if (blockIdx.z == 0 && g == 0 && row0 + 16 * t + c < rows) dots[at] = D[t];
+            if (split == 0 && g == 0 && row0 + 16 * t + c < rows) dots[at] = D[t];
             sums[t] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) acc[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -209,8 +209,8 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
             const int i = call.group(row), h = hk * G + (row - i * G);
             const int64_t all = a.num_queries * a.heads, at = (qs.at + i) * a.heads + h;
             if (part) {
-                const int64_t mine = blockIdx.z * all + at;
-                float* stat = part + (int64_t)gridDim.z * all * C;
+                const int64_t mine = split * all + at;
+                float* stat = part + (int64_t)splits * all * C;
                 if (slopes && g == 0) {
                     stat[3 * mine] = st;
                     stat[3 * mine + 1] = spd;
@@ -247,14 +247,14 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         zero_rest(grad_v, a.k_ptr, a.num_graphs, a.num_nodes, (int64_t)a.kv_heads * C, blockIdx.x - call.blocks);
         return;
     }
-    const int tile0 = call.units(work_of<DIST>(call)), of = work_of<DIST>(call) - tile0 * call.units.by;
-    const int b = call.kv(of), hk = of - b * a.kv_heads;
+    const Work work = work_of<DIST>(call);
+    const int b = work.graph, hk = work.head, split = work.split, splits = call.splits.by;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
     int first = 0, last = rows;
-    if (gridDim.z > 1) {
-        const int each = ((rows + RT - 1) / RT + gridDim.z - 1) / gridDim.z * RT;
-        first = min((int64_t)rows, (int64_t)blockIdx.z * each);
+    if (splits > 1) {
+        const int each = ((rows + RT - 1) / RT + splits - 1) / splits * RT;
+        first = min((int64_t)rows, (int64_t)split * each);
         last = min((int64_t)rows, (int64_t)first + each);
     }
     const bool plain = !CAP && a.scale > 1e-18f;
@@ -265,7 +265,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         for (int h = lane; h < G; h += kWave) falls = falls && a.slope[hk * G + h] > 0.0f && a.slope[hk * G + h] < 1e18f;
     falls = __all(falls);
 
-    for (int tile = tile0; (int64_t)tile * kKeys < ks.n; tile += call.tiles) {
+    for (int tile = work.tile; (int64_t)tile * kKeys < ks.n; tile += call.tiles) {
         const int key0 = tile * kKeys + w * 16 * MK;
         frag<T> k[MK][kSteps], v[MK][kSteps];
         const float* dist[MK];
@@ -407,7 +407,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                 const int ch = 16 * x + 4 * g;
                 if (ch >= C) continue;
                 if (part) {   // [split][k, v][node, head, channel]
-                    float* mine = part + ((int64_t)blockIdx.z * 2 * all + at) * C + ch;
+                    float* mine = part + ((int64_t)split * 2 * all + at) * C + ch;
                     *reinterpret_cast<f32x4*>(mine) = gk[t][x];
                     *reinterpret_cast<f32x4*>(mine + all * C) = gv[t][x];
                 } else {
@@ -500,8 +500,8 @@ void launch_bwd(const Args& a, hipStream_t stream) {
     if (a.num_queries > 0) {
         const AttentionCut c = cut_bwd_q(a);
         float* part = c.splits > 1 ? split : nullptr;
-        const Call call = call_of(a, c.tiles);
-        const dim3 grid(call.blocks + kRestBlocks, 1, c.splits);
+        const Call call = call_of(a, c);
+        const dim3 grid(call.blocks + kRestBlocks);
         if (c.narrow)
             hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, M, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
                                want_slopes ? slopes : nullptr, part);
@@ -527,8 +527,8 @@ void launch_bwd(const Args& a, hipStream_t stream) {
     if (a.num_nodes > 0) {
         const AttentionCut c = cut_bwd_kv(a);
         float* part = c.splits > 1 ? split : nullptr;
-        const Call call = call_of(a, c.tiles);
-        const dim3 grid(call.blocks + kRestBlocks, 1, c.splits);
+        const Call call = call_of(a, c);
+        const dim3 grid(call.blocks + kRestBlocks);
         if (c.narrow)
             hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, MK, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
                                part);

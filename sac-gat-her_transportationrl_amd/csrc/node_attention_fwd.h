@@ -31,20 +31,20 @@ attention_fwd_kernel(Call call, float* part) {
         if (!part) zero_rest(out, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
         return;
     }
-    const int tile0 = call.units(work_of<DIST>(call)), unit = work_of<DIST>(call) - tile0 * call.units.by;
-    const int b = call.kv(unit), hk = unit - b * a.kv_heads;
+    const Work work = work_of<DIST>(call);
+    const int b = work.graph, hk = work.head, split = work.split, splits = call.splits.by;
     const Span qs = span(a.q_ptr, b, a.num_queries), ks = span(a.k_ptr, b, a.num_nodes);
     const int rows = qs.n * G;
     int first = 0, last = ks.n;
-    if (gridDim.z > 1) {
-        const int each = ((ks.n + KT - 1) / KT + gridDim.z - 1) / gridDim.z * KT;
-        first = min((int64_t)ks.n, (int64_t)blockIdx.z * each);
+    if (splits > 1) {
+        const int each = ((ks.n + KT - 1) / KT + splits - 1) / splits * KT;
+        first = min((int64_t)ks.n, (int64_t)split * each);
         last = min(ks.n, first + each);
     }
     const T* k_base = static_cast<const T*>(a.k) + ks.at * a.k_row + hk * a.k_head;
     const T* v_base = static_cast<const T*>(a.v) + ks.at * a.v_row + hk * a.v_head;
 
-    for (int tile = tile0; (int64_t)tile * kRows < rows; tile += call.tiles) {
+    for (int tile = work.tile; (int64_t)tile * kRows < rows; tile += call.tiles) {
         const int row0 = tile * kRows + w * 16 * MQ;
         Staged<T, CP, KT, kThreads> k_next, v_next;
         auto fetch = [&](int j0) {
@@ -176,8 +176,8 @@ attention_fwd_kernel(Call call, float* part) {
             const int i = call.group(row), h = hk * G + (row - i * G);
             const int64_t at = (qs.at + i) * a.heads + h;
             if (part) {   // this split's sum and accumulator, for attention_join_kernel
-                const int64_t all = a.num_queries * a.heads, mine = blockIdx.z * all + at;
-                float* stat = part + (int64_t)gridDim.z * all * C;
+                const int64_t all = a.num_queries * a.heads, mine = split * all + at;
+                float* stat = part + (int64_t)splits * all * C;
                 if (g == 0) {
                     stat[2 * mine] = m[t];
                     stat[2 * mine + 1] = sum;
@@ -274,8 +274,8 @@ template <typename T, int CP, bool DIST, bool CAP>
 void launch_fwd(const Args& a, hipStream_t stream) {
     const AttentionCut c = cut_fwd(a);
     float* part = c.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
-    const Call call = call_of(a, c.tiles);
-    const dim3 grid(call.blocks + kRestBlocks, 1, c.splits);
+    const Call call = call_of(a, c);
+    const dim3 grid(call.blocks + kRestBlocks);
     constexpr int kWide = sizeof(T) == 2 && CP <= 64 ? 64 : 32;
     if (!c.narrow)
         hipLaunchKernelGGL((attention_fwd_kernel<T, CP, kTilesOfWave<T, CP>, 4, kWide, DIST, CAP>), grid, dim3(256), 0,
