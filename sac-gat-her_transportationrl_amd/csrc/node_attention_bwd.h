@@ -269,6 +269,9 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         const int key0 = tile * kKeys + w * 16 * MK;
         frag<T> k[MK][kSteps], v[MK][kSteps];
         const float* dist[MK];
+        uint32_t d_off[MK];
+        // (16 n + 4 g + r) / G = 16 n / G + 4 g / G + r / G for every power of two up to 16; r0 is a multiple of 32
+        const bool steps = DIST && WAVES > 1 && 16 % G == 0 && a.dist_row < (1 << 22) && a.dist_cols >= ks.n;
         f32x4 gk[MK][CP / 16], gv[MK][CP / 16];
 #pragma unroll
         for (int t = 0; t < MK; ++t) {
@@ -281,7 +284,10 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                 k[t][s] = in ? load_frag(pk + 32 * s + 8 * g) : zero_frag<T>();
                 v[t][s] = in ? load_frag(pv + 32 * s + 8 * g) : zero_frag<T>();
             }
-            if (DIST) dist[t] = j < a.dist_cols ? a.dist + b * a.dist_graph + j : nullptr;
+            if (DIST) {
+                dist[t] = j < a.dist_cols ? a.dist + b * a.dist_graph + j : nullptr;
+                d_off[t] = call.group(4 * g) * (uint32_t)a.dist_row + j;
+            }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) gk[t][x] = gv[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -314,16 +320,29 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         for (int r0 = first; r0 < last; r0 += RT) {
             if (!kAhead) fetch(r0);
             if (DIST && key0 < ks.n) {
+                if (steps && r0 + RT <= rows && call.group(r0 + RT - 1) < a.dist_rows) {
+                    // rows in equal steps and all there: one 32-bit offset a lane, the rest is scalar
+                    const float* base = a.dist + b * a.dist_graph + (int64_t)call.group(r0) * a.dist_row;
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
+                    for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int row = min(r0 + 16 * n + 4 * g + r, rows - 1), i = call.group(row);
-                        const int64_t at = i * a.dist_row;
-                        const bool in = i < a.dist_rows;
+                        for (int r = 0; r < 4; ++r) {
+                            const float* row = base + (int64_t)call.group(16 * n + r) * a.dist_row;
 #pragma unroll
-                        for (int t = 0; t < MK; ++t) d[t][n][r] = in && dist[t] ? dist[t][at] : INFINITY;
-                    }
+                            for (int t = 0; t < MK; ++t) d[t][n][r] = row[d_off[t]];
+                        }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int row = min(r0 + 16 * n + 4 * g + r, rows - 1), i = call.group(row);
+                            const int64_t at = i * a.dist_row;
+                            const bool in = i < a.dist_rows;
+#pragma unroll
+                            for (int t = 0; t < MK; ++t) d[t][n][r] = in && dist[t] ? dist[t][at] : INFINITY;
+                        }
+                }
             }
             __syncthreads();
             q_next.store(q_tile);
