@@ -1369,6 +1369,7 @@ int check_attention(const trx_node_attention_args* a, bool backward) {
         if (a->num_queries > 0 && (!a->lse || !a->grad_out || !a->grad_q))
             return fail(TRX_EINVAL, "node_attention: NULL lse / grad_out / grad_q");
         if (a->num_nodes > 0 && (!a->grad_k || !a->grad_v)) return fail(TRX_EINVAL, "node_attention: NULL grad_k / grad_v");
+        if (a->grad_slope && (!a->slope || !a->dist)) return fail(TRX_EINVAL, "node_attention: grad_slope without slope and dist");
     }
     const size_t need = trx::node_attention_workspace(*a, backward);
     if (need > 0 && (!a->workspace || a->workspace_bytes < (int64_t)need))

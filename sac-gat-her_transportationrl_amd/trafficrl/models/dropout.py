@@ -71,7 +71,8 @@ def dropout_add(x: torch.Tensor, rng: torch.Tensor, p: float, *, residual: Optio
 
     Differentiable once in x and residual; the pair in use is kept with the
     graph, so rng may move on before the backward pass.  Computed in float32,
-    rounded once."""
+    rounded once.  Asynchronous on the current stream and capturable; before a
+    backward pass is captured, drop the eager graphs of the same leaves."""
     what = "dropout_add"
     code = _lib.float_code(x, f"{what}: x")
     border = int(math.floor(float(p) * 65536.0 + 0.5)) if math.isfinite(p) else -1

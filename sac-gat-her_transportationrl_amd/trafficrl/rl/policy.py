@@ -99,7 +99,9 @@ def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Option
     or +inf that may be chosen has NaN for its values.
 
     Differentiable once in logits through log_prob, entropy and top_log_prob.
-    Computed in float32 (the gradient rounded once to the logits' type)."""
+    Computed in float32 (the gradient rounded once to the logits' type).
+    Asynchronous on the current stream and capturable; before a backward pass is
+    captured, drop the eager graphs of the same leaves."""
     what = "action_log_probs"
     code = _lib.float_code(logits, f"{what}: logits")
     if row_ptr is None:

@@ -119,7 +119,7 @@ def _attention_args():
     ("scale", math.nan, -1), ("cap", -1.0, -1), ("cap", 1e-35, -1), ("q", None, -1), ("v", None, -1), ("q_ptr", None, -1),
     ("k_ptr", None, -1), ("out", None, -1), ("q", 4100, -1), ("k_row", 65, -1), ("v_head", -32, -1),
     ("lse", None, -1), ("grad_out", None, -1), ("grad_k", None, -1), ("grad_v", 4104, -1),
-    ("workspace", None, -1), ("workspace_bytes", 4, -1), ("workspace", 4100, -1)])
+    ("grad_slope", 4096, -1), ("workspace", None, -1), ("workspace_bytes", 4, -1), ("workspace", 4100, -1)])
 def test_attention_boundary(field, value, code):
     from trafficrl import _lib
     L = _lib.load()
