@@ -8,11 +8,17 @@
 // rows of every head that shares them (grad_k, grad_v).  Seven products where
 // five would do, for results that do not depend on the order of anything.
 //
-// What bounds them: as forward, the scores' vector instructions (16 and 18 issue
-// slots a score) with two waves a SIMD, the most that operands and accumulators
-// leave registers for.  4001 nodes, 8 heads of 64, bfloat16, distances: 130 us
-// (grad_q) and 145 us (grad_k, grad_v), 290 TFLOP/s of the five products that are
-// needed; 4096 nodes without distances 192 us together (450 TFLOP/s).
+// D = <grad_out, out> is subtracted from <grad_out, v>, and its error does not
+// shrink with the difference.  out alone, rounded to bfloat16, leaves grad_q off by
+// 0.0041 (relative to float64) where all values are shifted by 1, 0.0139 by 4,
+// 0.0042 where the softmax is peaked; with out_low 0.0024 to 0.0025.  Inputs of
+// mean zero gain nothing.  out_low costs 0.5 us forward and 2 us here at 4001 nodes.
+//
+// What bounds them: as forward, vector instructions (12.7 and 13.8 a score, issuing
+// in 45% and 38% of the cycles, the matrix pipe busy in 20%) and waiting, with two
+// waves a SIMD.  4001 nodes, 8 heads of 64, bfloat16, distances: 134 us (grad_q) and
+// 150 us (grad_k, grad_v), 288 TFLOP/s of the five products that are needed; 4096
+// nodes without distances 189 us together with the sums (455 TFLOP/s).
 #pragma once
 #include <algorithm>
 
@@ -236,8 +242,8 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     }
 }
 
-// Distances here are read where they are used: a fragment's sixteen lanes lie along a row already (through LDS: 157
-// against 160 us at 4096 nodes, 184 against 161 at 4001).
+// Distances are read where they are used: a fragment's sixteen lanes lie along a row already.  Staged through LDS as
+// in the other passes this one took 184 us at 4001 nodes; it took 157 us once that and some of its score code went.
 template <typename T, int CP, int MK, int WAVES, int RT, bool DIST, bool CAP>
 __global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, CP, WAVES>)))
 attention_bwd_kv_kernel(Call call, const float* dots, float* part) {

@@ -7,17 +7,16 @@
 // of the group), so a shared head's keys are read once.  Keys, values and
 // distances pass through LDS in tiles of KT, the next tile on its way in registers.
 //
-// What bounds it.  Large graphs: the vector instructions of the scores (a
-// multiply-add for the distance, one for the exponent, exp at a quarter of the
-// rate, the sum, the rounding: some 13 issue slots a score with the tile's
-// overhead), about as long as the matrix instructions at 128 channels and twice
-// as long at 64.  4096 nodes, 8 heads, bfloat16: 111 us at 128 channels (620
-// TFLOP/s), 75 us at 64 (455); with distances 140 and 107 us.  Two waves a SIMD
-// is what registers allow; tiles of 64 keys at 64 channels, of 32 at 128 (64 keys
-// at 64 channels with distances: 107 us, 32 keys: 120 us).  Small graphs and
-// single queries: memory.  4096 networks of 24 nodes, 4 heads of 64: 42 us (201
-// MB at 4.8 TB/s, a large copy's rate); 8 queries over 32768 nodes each, 16 heads
-// on 2 of 128: 50 us and 7 us for joining 64 splits (270 MB at 4.7 TB/s).
+// What bounds it.  Large graphs: the vector instructions of the scores and waiting.
+// 4096 nodes, 8 heads of 64, bfloat16, with distances: 10.7 vector instructions a
+// score issue in 47% of the cycles, the matrix pipe is busy in 16%; registers
+// allow two waves a SIMD (three: 183 us against 132 when tried).  Times at 4096
+// nodes, 8 heads, bfloat16: 110 us at 128 channels (628 TFLOP/s), 76 at 64 (452);
+// with distances 142 and 107.  64 keys a tile at 64 channels with distances (32:
+// 120 us against 107), 32 at 128.  Small graphs and single queries: memory.  4096
+// networks of 24 nodes, 4 heads of 64: 42 us (201 MB at 4.8 TB/s, a large copy's
+// rate); 8 queries over 32768 nodes each, 16 heads on 2 of 128: 50 us and 7 us for
+// joining the splits (270 MB at 4.7 TB/s together).
 #pragma once
 #include <algorithm>
 
