@@ -22,8 +22,12 @@ AttentionCut cut(int64_t kept, int64_t run, int64_t all, int64_t graphs, int64_t
     c.narrow = kept <= 32;
     c.mq = c.narrow && kept <= 16 ? 1 : 2;
     const int64_t each = c.narrow ? 16 * c.mq : wide;
-    c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, (1 << 23) / units));
-    const int64_t blocks = std::max<int64_t>(1, std::min(units * c.tiles, heads * (all / each + graphs)));
+    // Workgroups of no rows cost 0.9 us a thousand: no more of them than four times those that can have rows, or 2^17
+    // in all; a graph's further tiles are looped over.  4096 graphs of 24 nodes whose largest is not known: UNHINTED.
+    const int64_t filled = heads * (all / each + graphs);
+    const int64_t limit = std::min<int64_t>(1 << 23, std::max<int64_t>(1 << 17, 4 * filled));
+    c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, limit / units));
+    const int64_t blocks = std::max<int64_t>(1, std::min(units * c.tiles, filled));
     const int64_t want = c.narrow ? 2048 : 512;
     const int64_t most = std::min<int64_t>(64, std::min(run / least, (int64_t(1) << 28) / std::max<int64_t>(1, row_bytes)));
     c.splits = (int)std::max<int64_t>(1, std::min((want + blocks - 1) / blocks, most));

@@ -280,3 +280,23 @@ def test_beyond_32_bits():
     r = action_log_probs(x, a, row_ptr=ptr, max_row=200, top_k=4)
     s = action_log_probs(x[-300:].clone(), a, row_ptr=torch.tensor([0, 200, 300], device="cuda"), max_row=200, top_k=4)
     assert all(torch.equal(u, v) for u, v in zip(r, s))
+
+
+def test_many_short_rows_and_a_long_one():
+    """More rows than a launch has workgroups for: the long row's further chunks
+    are looped over; without the hint the same bits as alone, links in order."""
+    from trafficrl.rl import action_log_probs
+    many, n = 40000, 50001
+    g = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(3 * many + n, device="cuda", generator=g)
+    ptr = torch.cat([torch.arange(many + 1, device="cuda") * 3, torch.tensor([3 * many + n], device="cuda")])
+    act = torch.zeros(many + 1, dtype=torch.int64, device="cuda")
+    act[-1] = n - 1
+    y = x.clone().requires_grad_()
+    r = action_log_probs(y, act, row_ptr=ptr)
+    grad, = torch.autograd.grad(r.log_prob.sum(), y)
+    # float64, and the bounds: exp, sums of n terms in any order and the division, each 2^-24 relative to values <= 1
+    for part, rows, links in ((slice(0, 3 * many), many, 3), (slice(3 * many, None), 1, n)):
+        p = torch.softmax(x[part].double().view(rows, links), 1)
+        onehot = torch.nn.functional.one_hot(act[:many] if rows > 1 else act[-1:], links)
+        assert ((grad[part].view(rows, links) - (onehot - p)).abs() <= (links + 64) * U).all()

@@ -347,3 +347,34 @@ def test_long_offsets():
     view.copy_(x)
     p = ints([0, 17, rows])
     assert torch.equal(node_attention(x, view, view, p), node_attention(x, x, x, p))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=str)
+def test_many_small_networks_and_a_large_one(dt):
+    """More networks than a launch has tiles for: the large one's further tiles
+    are looped over, whether the hints say so or not."""
+    from trafficrl.models import node_attention
+    many, n, H, C = 40000, 700, 4, 16
+    g = torch.Generator("cuda").manual_seed(11)
+    rnd = lambda: torch.randn(many + n, H, C, device="cuda", generator=g).to(dt)  # noqa: E731
+    q, k, v, go = rnd(), rnd(), rnd(), rnd()
+    dist = torch.rand(n, n, device="cuda", generator=g) * 6
+    ptr = torch.arange(many + 2, device="cuda")
+    ptr[-1] = many + n
+    # A single node sees itself: out = v, grad_v = go, up to p = 2^(w - statistics), which is 1 only if w is the same in
+    # both.  attention_reference's bounds with n = 1 and M the largest scale sum |q||k| (scores and statistics are
+    # below M): dw <= (C + 1) u M + 12 u M, p off by 2 dw + 9 u, the result by 9 u more, and by the type's roundings
+    # of p (2 h) and of the result (h).
+    M = float((q.double() * k.double()).abs().sum(-1).max()) / math.sqrt(C)
+    h = {F32: 0.0, BF16: 2.0 ** -8}[dt]
+    near = 2 * (C + 13) * 2.0 ** -24 * max(M, 1.0) + 18 * 2.0 ** -24 + 3 * h
+    want = reference(q[many:], k[many:], v[many:], [0, n], [0, n], dist, None, None, 0.0, go[many:])
+    for hints in ({}, {"max_queries": n, "max_nodes": n}):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = node_attention(*leaves, ptr, dist=dist, **hints)
+        grads = torch.autograd.grad(out, leaves, go)
+        for got, own in ((out, v), (grads[2], go)):
+            assert ((got[:many].double() - own[:many].double()).abs() <= near * own[:many].double().abs()).all()
+        assert_within("out", out[many:], *want["out"])
+        for name, t in zip("qkv", grads):
+            assert_within(name, t[many:], *want[name])
