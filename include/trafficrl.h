@@ -880,7 +880,7 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
  * log2(sum_j 2^(w log2 e)), written by the forward where not NULL (-inf for an
  * empty row), read by the backward.  out_low: like out, or NULL: what rounding
  * took from out; with it the backward's <grad_out, out> is as exact as in
- * float32.  grad_slope float32 [heads] or NULL.
+ * float32.  grad_slope float32 [heads] or NULL (NULL without slope or dist).
  * max_queries / max_nodes: the largest graph's rows; they only shape the
  * launch (a smaller value costs time, never rows).  Sums and the softmax's
  * statistics are float32; probabilities and score gradients enter the matrix

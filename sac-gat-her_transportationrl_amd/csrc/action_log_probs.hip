@@ -611,7 +611,8 @@ hipError_t launch_action_log_probs_bwd(const trx_action_log_probs_args& a, hipSt
             hipLaunchKernelGGL(log_probs_short_bwd_kernel<T>, dim3(blocks + rest), dim3(kThreads), 0, stream, a, blocks);
         } else {
             // packed rows may be much shorter than the longest (or than `max_row` says): about 2^15 workgroups then, which
-            // loop over a row's further chunks; a chunk each would be rows x total of them.  (measured)
+            // loop over a row's further chunks; a chunk each would be rows x total of them (32768 rows of
+            // 76, longest not given: 2747 us, 137 now, 61 where it is given).
             const int64_t most = a.row_ptr ? std::max<int64_t>(1, (1 << 15) / std::max<int64_t>(1, a.rows)) : 65535;
             const unsigned chunks = (unsigned)std::min<int64_t>((n + kChunk - 1) / kChunk, std::min<int64_t>(most, 65535));
             hipLaunchKernelGGL(log_probs_long_bwd_kernel<T>, dim3((unsigned)a.rows + (a.row_ptr ? 1 : 0), chunks),

@@ -23,7 +23,8 @@ AttentionCut cut(int64_t kept, int64_t run, int64_t all, int64_t graphs, int64_t
     c.mq = c.narrow && kept <= 16 ? 1 : 2;
     const int64_t each = c.narrow ? 16 * c.mq : wide;
     // Workgroups of no rows cost 0.9 us a thousand: no more of them than four times those that can have rows, or 2^17
-    // in all; a graph's further tiles are looped over.  4096 graphs of 24 nodes whose largest is not known: UNHINTED.
+    // in all; a graph's further tiles are looped over.  4096 graphs of 24 nodes and 4 heads whose
+    // largest is not given: forward 360 us, 7525 with up to 2^23 workgroups, 43 where it is given.
     const int64_t filled = heads * (all / each + graphs);
     const int64_t limit = std::min<int64_t>(1 << 23, std::max<int64_t>(1 << 17, 4 * filled));
     c.tiles = std::max<int64_t>(1, std::min<int64_t>((kept + each - 1) / each, limit / units));

@@ -90,7 +90,8 @@ def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Option
     most 2^30 links in a row).  action: int64 [rows], row-local.  mask: shaped like
     logits; a link may be chosen where it is > 0 (the env's action_mask; bool
     works too).  A logit of -inf is a link that may not be chosen; large negative
-    fills are ordinary logits.  max_row: the longest row of a packed batch, a hint.
+    fills are ordinary logits.  max_row: the longest row of a packed batch, a
+    hint that makes many short rows faster.
     top_k: 0 (top_* are None) .. 16.
 
     An action that may not be chosen, or lies outside its row, has log probability
