@@ -130,3 +130,75 @@ def test_second_derivatives_are_refused():
         assert torch.equal(g, want)
         with pytest.raises(RuntimeError, match="once, not twice"):
             ((g * g).sum() + leaf.sum()).backward()
+
+
+def test_broadcast_inputs_and_one_leaf_in_several_places():
+    """Inputs of stride zero, and a leaf that is query, key, value and residual:
+    the gradients add up to those of separate copies."""
+    from trafficrl.models import dropout_add, node_attention
+    from trafficrl.rl import action_log_probs
+    g = torch.Generator("cuda").manual_seed(21)
+    ptr = torch.tensor([0, 20, 50], device="cuda")
+    one = torch.randn(50, 1, 32, device="cuda", generator=g).requires_grad_()
+    s1 = torch.rand(1, device="cuda", generator=g).requires_grad_()
+    d1 = torch.rand(1, 30, device="cuda", generator=g).expand(30, 30)     # every row alike
+    go = torch.randn(50, 4, 32, device="cuda", generator=g)
+
+    def attend(q, k, v, s, d):
+        return node_attention(q, k, v, ptr, dist=d, slope=s)
+    wide = one.expand(50, 4, 32)
+    got = torch.autograd.grad(attend(wide, wide, wide, s1.expand(4), d1), [one, s1], go)
+    parts = [one.detach().expand(50, 4, 32).clone().requires_grad_() for _ in range(3)]
+    s4 = s1.detach().expand(4).clone().requires_grad_()
+    apart = torch.autograd.grad(attend(*parts, s4, d1.contiguous()), [*parts, s4], go)
+    # the same bits three times over, added in another order: 12 terms and 4 terms of float32
+    want = sum(t.double() for t in apart[:3]).sum(1, keepdim=True)
+    size = sum(t.double().abs() for t in apart[:3]).sum(1, keepdim=True)
+    assert ((got[0].double() - want).abs() <= 12 * 2.0 ** -24 * size).all()
+    assert abs(float(got[1].double() - apart[3].double().sum())) <= 4 * 2.0 ** -24 * float(apart[3].double().abs().sum())
+
+    row = torch.randn(1, 76, device="cuda", generator=g).requires_grad_()
+    mask = (torch.rand(1, 76, device="cuda", generator=g) > 0.3).expand(9, 76)
+    action = torch.randint(0, 76, (9, 3), device="cuda", generator=g)[:, 1]
+    a = action_log_probs(row.expand(9, 76), action, mask=mask, top_k=3)
+    many = row.detach().expand(9, 76).clone().requires_grad_()
+    b = action_log_probs(many, action.contiguous(), mask=mask.contiguous(), top_k=3)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    w = torch.randn(9, device="cuda", generator=g)
+    ga, = torch.autograd.grad(a.entropy, row, w)
+    gb, = torch.autograd.grad(b.entropy, many, w)
+    assert ((ga.double() - gb.double().sum(0)).abs() <= 9 * 2.0 ** -24 * gb.double().abs().sum(0)).all()
+
+    rng = torch.tensor([3, 4], device="cuda")
+    x = torch.randn(40, 33, device="cuda", generator=g).requires_grad_()
+    gx, = torch.autograd.grad(dropout_add(x, rng, 0.25, residual=x), x, torch.ones(40, 33, device="cuda"))
+    kept = dropout_add(torch.ones(40, 33, device="cuda"), rng, 0.25)
+    assert torch.equal(gx, kept + 1)
+
+
+def test_two_streams_at_once():
+    """The same operators on two streams share nothing: the bits of one after the other."""
+    from trafficrl.models import node_attention
+    from trafficrl.rl import action_log_probs
+    g = torch.Generator("cuda").manual_seed(22)
+    ptr = torch.tensor([0, 700], device="cuda")
+    sets = [[torch.randn(700, 2, 64, device="cuda", generator=g).bfloat16().requires_grad_() for _ in range(3)]
+            for _ in range(2)]
+    go = torch.randn(700, 2, 64, device="cuda", generator=g).bfloat16()
+    rows = [torch.randn(3, 50001, device="cuda", generator=g) for _ in range(2)]
+    action = torch.tensor([0, 7, 50000], device="cuda")
+
+    def run(i):
+        out = node_attention(*sets[i], ptr)
+        return [out.detach(), *torch.autograd.grad(out, sets[i], go), *action_log_probs(rows[i], action, top_k=8)]
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, run(i)))
+    torch.cuda.synchronize()
+    for i, r in got:
+        assert all(torch.equal(x, y) for x, y in zip(r, want[i]))
