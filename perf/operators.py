@@ -22,12 +22,10 @@ DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch
 SIZE = {"float32": 4, "bfloat16": 2, "float16": 2}
 
 
-PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sac-gat-her_transportationrl_amd")
-
-
 def _package():
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sac-gat-her_transportationrl_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
 
 
 def attention(name, graphs, low, high, queries, heads, kv_heads, channels, dtype, dist, cap, train):
