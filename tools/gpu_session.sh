@@ -125,8 +125,6 @@ for s in "$@"; do
         disttests) step dist_tests 600 python -u -m pytest tests/test_dist_gpu.py -m gpu -x -v --timeout 300 --timeout-method thread ;;
         dist2) step bench_dist2 600 env TRX_DIST_BACKEND=gloo python -m torch.distributed.run --nnodes=1 --nproc-per-node 2 --master-addr 127.0.0.1 --master-port 29517 bench.py --gpus 2 --steps 44 --warmup 22 --no-cpu ;;
         branchprobe) step branch_probe3 300 python tools/branch_probe.py 3 && step branch_probe6 300 python tools/branch_probe.py 6 ;;
-        fu1) step fu1 150 env AMD_SERIALIZE_KERNEL=3 python -u -m pytest tests/test_fused_update.py -m gpu -x -v -s --timeout 60 --timeout-method thread -k vs_fp32_restatement ;;
-        mprobe) step multi_probe 150 python -u tools/multi_probe.py 5 && PROBE_STAGES=1 step multi_stages 150 python -u tools/multi_probe.py 5 ;;
         multi) step multi_tests 900 python -u -m pytest tests/test_fused_update.py tests/test_concurrent_update.py tests/test_sac_e2e.py tests/test_gat_infer.py tests/test_flat_adam.py -m gpu -x -v -s --timeout 300 --timeout-method thread &&
                TRX_UPD_MULTI=0 step upd_time_m0 300 python tools/upd_time.py && TRX_UPD_MULTI=1 step upd_time_m1 300 python tools/upd_time.py &&
                TRX_UPD_MULTI=0 step upd_time_m0b 300 python tools/upd_time.py && TRX_UPD_MULTI=1 step upd_time_m1b 300 python tools/upd_time.py ;;
