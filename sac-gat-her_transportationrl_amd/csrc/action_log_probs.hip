@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kWave * kWaves) log_probs_join_kernel(Args a, 
 // What a row's gradient needs.  Lane 0 holds the action and its incoming gradient, lanes 1 .. top_k the alternatives
 // and theirs (link -1: none): the links that get more than their share of the sums.
 struct Grad {
-    float norm, entropy, all, g2;   // m + log s, the entropy, the sum of the incoming log probability gradients
+    float m, ls, entropy, all, g2;   // m, log s, the entropy, the sum of the incoming log probability gradients
     int64_t link;
     float extra;
 };
@@ -455,7 +455,8 @@ __device__ __forceinline__ Grad grad_of(const Args& a, int64_t r, int lane) {
     const float* st = a.stats + 4 * r;
     Grad g;
     g.entropy = st[2];
-    g.norm = st[0] + st[1];
+    g.m = st[0];
+    g.ls = st[1];
     g.g2 = a.g_entropy ? a.g_entropy[r] : 0.0f;
     g.link = -1;
     g.extra = 0.0f;
@@ -470,7 +471,9 @@ __device__ __forceinline__ Grad grad_of(const Args& a, int64_t r, int lane) {
     return g;
 }
 __device__ __forceinline__ float base_grad(const Grad& g, float x) {
-    const float lp = x - g.norm, p = __builtin_amdgcn_exp2f(lp * kLog2e);
+    // in two steps as forward: m + log s in one float would lose log s where |m| is large (a row whose links all hold
+    // the same -1e9 would get p = 1 for each of them)
+    const float lp = x - g.m - g.ls, p = __builtin_amdgcn_exp2f(lp * kLog2e);
     // where p is 0, lp may be -inf; a link that may not be chosen gets 0 in a row of NaN too
     const float d = -p * __builtin_fmaf(g.g2, fmaxf(lp, -1e30f) + g.entropy, g.all);
     return x == -INFINITY ? 0.0f : d;
