@@ -36,8 +36,9 @@ def _args(logits, mask, row_ptr, action, rest, outs, grads=(0, 0, 0, 0)):
 def _launch(logits, mask, row_ptr, action, rest):
     L, top_k, dev = _lib.load(), rest[1], logits.device
     n = action.shape[0]
-    log_prob, entropy, stats = torch.empty(n, device=dev), torch.empty(n, device=dev), torch.empty(n, 4, device=dev)
-    top_log_prob = torch.empty(n, top_k, device=dev) if top_k else None
+    floats = lambda *shape: torch.empty(shape, device=dev, dtype=torch.float32)  # noqa: E731
+    log_prob, entropy, stats = floats(n), floats(n), floats(n, 4)
+    top_log_prob = floats(n, top_k) if top_k else None
     top_action = torch.empty(n, top_k, device=dev, dtype=torch.int64) if top_k else None
     a = _args(logits, mask, row_ptr, action, rest, (log_prob, entropy, stats, top_log_prob, top_action))
     need = L.trx_action_log_probs_workspace_bytes(a)
@@ -50,7 +51,7 @@ def _launch(logits, mask, row_ptr, action, rest):
 
 
 def _launch_backward(logits, mask, row_ptr, action, stats, top_action, rest, grads):
-    grads = [None if t is None else t.contiguous() for t in grads]
+    grads = [None if t is None else t.contiguous() for t in grads]   # float32, like the outputs
     grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
     a = _args(logits, mask, row_ptr, action, rest, (None, None, stats, None, top_action),
               (*(0 if t is None else t.data_ptr() for t in grads), grad.data_ptr()))

@@ -1,0 +1,69 @@
+"""Calls of node_attention, dropout_add and action_log_probs that their
+documentation allows and ordinary programs make rarely: other default types,
+views whose strides say nothing, sizes at the limits, forward-mode tangents."""
+import math
+
+import pytest
+import torch
+
+
+class _Recorder:
+    """Stands in for the library on a CPU: every entry succeeds and does nothing."""
+
+    def __getattr__(self, name):
+        return lambda *a: 0
+
+
+@pytest.fixture
+def no_library(monkeypatch):
+    from trafficrl import _lib
+    monkeypatch.setattr(_lib, "load", lambda: _Recorder())
+    monkeypatch.setattr(_lib, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(_lib, "same_device", lambda what, first, *others: None)
+    monkeypatch.setattr(_lib, "on_device", lambda device, f, *a: f(*a))
+
+
+@pytest.fixture(params=[torch.float64, torch.float32, torch.float16, torch.bfloat16], ids=str)
+def default_dtype(request):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(request.param)
+    yield request.param
+    torch.set_default_dtype(before)
+
+
+def test_buffers_have_the_kernels_types(no_library, default_dtype):
+    """Whatever torch's default type is: a two-byte one would leave the kernels half the memory that they write."""
+    from trafficrl.models import dropout_add, node_attention
+    from trafficrl.rl import action_log_probs
+    logits = torch.zeros(3, 9, dtype=torch.float32, requires_grad=True)
+    r = action_log_probs(logits, torch.zeros(3, dtype=torch.int64), top_k=2)
+    assert r.log_prob.dtype == r.entropy.dtype == r.top_log_prob.dtype == torch.float32
+    assert r.top_action.dtype == torch.int64
+    saved = r.log_prob.grad_fn.saved_tensors
+    stats = [t for t in saved if t is not None and t.shape == (3, 4)]
+    assert len(stats) == 1 and stats[0].dtype == torch.float32
+    q = torch.zeros(6, 2, 32, dtype=torch.bfloat16, requires_grad=True)
+    out = node_attention(q, q, q, torch.tensor([0, 6]))
+    assert out.dtype == torch.bfloat16
+    lse = [t for t in out.grad_fn.saved_tensors if t is not None and t.shape == (6, 2)]
+    assert len(lse) == 1 and lse[0].dtype == torch.float32
+    assert dropout_add(q, torch.zeros(2, dtype=torch.int64), 0.5).dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+def test_default_type_does_not_matter():
+    from trafficrl.rl import action_log_probs
+    x = torch.randn(5, 76, device="cuda")
+    a = torch.arange(5, device="cuda")
+
+    def both():
+        leaf = x.clone().requires_grad_()
+        r = action_log_probs(leaf, a, top_k=3)
+        return [*r, *torch.autograd.grad(r.log_prob.sum() + r.entropy.sum(), leaf)]
+    want = both()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = both()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(s, t) and s.dtype == t.dtype for s, t in zip(want, got))
