@@ -16,11 +16,13 @@ def _strided(t: torch.Tensor) -> torch.Tensor:
     """t itself where the kernels can read it (channels contiguous, rows and
     heads 16-byte aligned), else a contiguous copy."""
     unit = 16 // t.element_size()
+    for dim in (1, 0):   # a dimension of one may have any stride, and contiguous() would leave it
+        if t.shape[dim] == 1 and t.stride(dim) % unit:
+            t = t.squeeze(dim).unsqueeze(dim)
     s = t.stride()
     if s[2] == 1 and s[0] % unit == 0 and s[1] % unit == 0 and t.data_ptr() % 16 == 0:
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _args(q, k, v, ptr, k_ptr, dist, slope, rest, out, low, lse, backward: bool, grads=(0, 0, 0, 0, 0)):

@@ -67,3 +67,41 @@ def test_default_type_does_not_matter():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(torch.equal(s, t) and s.dtype == t.dtype for s, t in zip(want, got))
+
+
+def _odd_strides(rows, heads, channels, dt, **kw):
+    """Tensors with a dimension of one whose stride is no multiple of 16 bytes and never used."""
+    base = torch.randn(4096, **kw).to(dt)
+    if rows == 1:      # one row of a wider one
+        yield base.as_strided((1, heads, channels), (heads * channels + 3, channels, 1), 0)
+    if heads == 1:     # one head out of a layout with heads innermost but one
+        yield base.as_strided((rows, 1, channels), (channels, 5, 1), 0)
+        yield base.as_strided((rows, 1, channels), (channels + 8, 7, 1), 8)
+    yield base.as_strided((rows, heads, channels), (heads * channels, channels, 1), 1)   # not aligned
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 4), (1, 1), (6, 1)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_dimensions_of_one_have_any_stride(rows, heads, dt):
+    """contiguous() leaves such a stride as it is; the kernels' boundary takes multiples of 16 bytes."""
+    from trafficrl.models.attention import _strided
+    unit = 16 // torch.zeros(0, dtype=dt).element_size()
+    for t in _odd_strides(rows, heads, 32, dt):
+        s = _strided(t)
+        assert s.stride(2) == 1 and s.stride(0) % unit == 0 and s.stride(1) % unit == 0 and s.data_ptr() % 16 == 0
+        assert torch.equal(s, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,heads", [(1, 4), (1, 1), (6, 1)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=str)
+def test_attention_of_dimensions_of_one(rows, heads, dt):
+    from trafficrl.models import node_attention
+    p = torch.tensor([0, rows], device="cuda")
+    for t in _odd_strides(rows, heads, 32, dt, device="cuda"):
+        c = torch.empty(t.shape, device="cuda", dtype=dt).copy_(t)
+        leaf, plain = t.detach().requires_grad_(), c.requires_grad_()
+        a, b = node_attention(leaf, t, leaf, p), node_attention(plain, c.detach(), plain, p)
+        go = torch.randn(t.shape, device="cuda").to(dt)
+        assert torch.equal(a, b)
+        assert torch.equal(torch.autograd.grad(a, leaf, go)[0], torch.autograd.grad(b, plain, go)[0])
