@@ -885,7 +885,8 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
  * launch (a smaller value costs time, never rows).  Sums and the softmax's
  * statistics are float32; probabilities and score gradients enter the matrix
  * products in dtype.  Deterministic: no float atomics.  At most 2^23 / heads
- * graphs.  workspace:
+ * graphs, 2^31 - 2^16 nodes, and query rows x heads / kv_heads up to 2^31 - 256.
+ * workspace:
  * trx_node_attention_workspace_bytes(args, backward) bytes, 16-byte aligned
  * (0: may be NULL).                                                        */
 #define TRX_ATT_MAX_CHANNELS 128

@@ -1339,8 +1339,9 @@ int check_attention_shape(const trx_node_attention_args* a) {
                     TRX_ATT_MAX_CHANNELS, a->channels);
     if (a->num_queries > ((int64_t(1) << 31) - 256) / (a->heads / a->kv_heads))
         return fail(TRX_EUNSUP, "node_attention: query rows x heads of a group must stay below 2^31 - 256");
-    if (a->num_queries > (int64_t(1) << 31) - 1 || a->num_nodes > (int64_t(1) << 31) - 1)
-        return fail(TRX_EUNSUP, "node_attention: at most 2^31 - 1 rows");
+    // the kernels step over a graph's keys in 32 bits, a tile or a split's rounding behind the last one
+    if (a->num_nodes > (int64_t(1) << 31) - (1 << 16))
+        return fail(TRX_EUNSUP, "node_attention: at most 2^31 - 2^16 nodes");
     if ((int64_t)a->num_graphs + 1 > (1 << 23) / a->heads)
         return fail(TRX_EUNSUP, "node_attention: at most 2^23 / heads graphs");
     return TRX_OK;

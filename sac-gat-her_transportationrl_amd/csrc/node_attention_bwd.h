@@ -58,7 +58,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     if (splits > 1) {
         const int each = ((ks.n + KT - 1) / KT + splits - 1) / splits * KT;
         first = min((int64_t)ks.n, (int64_t)split * each);
-        last = min(ks.n, first + each);
+        last = min((int64_t)ks.n, (int64_t)first + each);
     }
     const T* k_base = static_cast<const T*>(a.k) + ks.at * a.k_row + hk * a.k_head;
     const T* v_base = static_cast<const T*>(a.v) + ks.at * a.v_row + hk * a.v_head;

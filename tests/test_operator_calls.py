@@ -105,3 +105,20 @@ def test_attention_of_dimensions_of_one(rows, heads, dt):
         go = torch.randn(t.shape, device="cuda").to(dt)
         assert torch.equal(a, b)
         assert torch.equal(torch.autograd.grad(a, leaf, go)[0], torch.autograd.grad(b, plain, go)[0])
+
+
+@pytest.mark.parametrize("nodes,code", [((1 << 31) - (1 << 16) + 1, -3), ((1 << 31) - 1, -3), (1 << 31, -3)])
+def test_nodes_below_the_kernels_counters(nodes, code):
+    """Keys (a stride of zero makes that many out of one) that a 32-bit counter would step over the end of."""
+    from test_operators_cpu import _attention_args
+    from trafficrl import _lib
+    L = _lib.load()
+    a = _attention_args()
+    a.num_nodes = a.max_nodes = nodes
+    a.workspace_bytes = 0     # never launched: without the limit the workspace's check refuses the call
+    a.workspace = None
+    assert L.trx_node_attention_forward(a, None) == code and L.trx_node_attention_backward(a, None) == code
+    assert b"nodes" in L.trx_last_error()
+    assert L.trx_node_attention_workspace_bytes(a, 0) == -1
+    a.num_nodes = a.max_nodes = (1 << 31) - (1 << 16)
+    assert L.trx_node_attention_workspace_bytes(a, 1) > 0
