@@ -877,8 +877,9 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
  * channels a multiple of 8 up to TRX_ATT_MAX_CHANNELS.  out, grad_out,
  * grad_q [num_queries, heads, channels], grad_k, grad_v [num_nodes, kv_heads,
  * channels]: contiguous, in dtype.  lse float32 [num_queries, heads]:
- * log2(sum_j 2^(w log2 e)), written by the forward where not NULL (-inf for an
- * empty row), read by the backward.  out_low: like out, or NULL: what rounding
+ * log(sum_j e^w), written by the forward where not NULL (-inf for an empty
+ * row), read by the backward, which sums the weights around it anew: what its
+ * rounding loses where a row's scores are large and alike does not count.  out_low: like out, or NULL: what rounding
  * took from out; with it the backward's <grad_out, out> is as exact as in
  * float32.  grad_slope float32 [heads] or NULL (NULL without slope or dist).
  * max_queries / max_nodes: the largest graph's rows; they only shape the

@@ -1,5 +1,5 @@
-// node_attention.h -- what the attention kernels share (node_attention.hip,
-// node_attention_bwd.hip): matrix fragments, staged tiles, scores.
+// node_attention.h -- what the attention kernels share (node_attention_fwd.h,
+// node_attention_bwd.h): matrix fragments, staged tiles, scores.
 //
 // Fragments.  The 16 x 16 matrix instructions take, in lane l (g = l / 16, c = l
 // % 16), eight operand elements of row or column c at depth 8g .. 8g+7 of a
@@ -16,6 +16,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "float_types.h"
@@ -34,7 +35,7 @@ struct AttentionCut {
 namespace {
 
 constexpr int kWave = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 using Args = trx_node_attention_args;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -157,16 +158,33 @@ inline Divide divide_by(int d) {
 // L2 where there are 8 k heads.  Where there are distances, the heads of a tile go to one die instead: they read the
 // same 4 bytes a pair and head, which would otherwise come through the fabric once a die.
 constexpr int kRestBlocks = 16;
+// What scores are counted in: a power of two, so that products with it are exact.  Natural units where a bias or a cap
+// comes in; else the power of two below the scale, so that a scale like 1 / 8 leaves the products as they come.
+struct Unit {
+    float pre;     // what the products <q, k> are multiplied by (where scores are capped: to the tanh's argument)
+    float log2;    // from scores to log 2
+    float nat;     // from scores to natural units, and back
+    float per;
+};
+inline Unit unit_of(const Args& a) {
+    if (a.cap > 0.0f) return {a.scale / a.cap, kLog2e, 1.0f, 1.0f};
+    if (a.dist) return {a.scale, kLog2e, 1.0f, 1.0f};
+    int e = a.scale == 0.0f ? 0 : std::ilogb(a.scale);
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    return {std::ldexp(a.scale, -e), std::ldexp(kLog2e, e), std::ldexp(1.0f, e), std::ldexp(1.0f, -e)};
+}
+
 struct Call {
     Args a;
     Divide group, kv, units;   // by heads of a group, key/value heads, (graph, key/value head)s
     Divide splits;
     int tiles, blocks;
+    Unit unit;
 };
 inline Call call_of(const Args& a, const AttentionCut& c) {
     const int units = a.num_graphs * a.kv_heads;
     return {a, divide_by(a.heads / a.kv_heads), divide_by(a.kv_heads), divide_by(units > 0 ? units : 1),
-            divide_by(c.splits), (int)c.tiles, (int)c.tiles * c.splits * units};
+            divide_by(c.splits), (int)c.tiles, (int)c.tiles * c.splits * units, unit_of(a)};
 }
 
 // one column's four distances behind key j: +inf from `limit` on
@@ -335,27 +353,26 @@ __device__ __forceinline__ float column_max(float v) {
     return fmaxf(v, __shfl_xor(v, 32));
 }
 
-// Scores w = scale x - slope d, unseen at -inf.  Where every lane's slope is
-// positive and the scale too (`plain`), they are kept divided by the scale: the
-// product with it joins the exponential's, and a distance of +inf makes its -inf
-// by itself, so one multiply-add a score is all.  Distances that are negative or
-// NaN anywhere in the tile, or other signs, take selects.
-struct Bias {
-    float slope;   // -slope / scale where plain, else -slope
-    float pre;     // what scores are multiplied by first
-    float unit;    // from the scores' unit to log 2
-    bool plain;
+// A row's weights are 2^(w unit - R) for some reference R near its largest score's.  Everything is divided by their sum in
+// the end, so R need not be anything in particular, but it must be the same number for each of them, and near: log2 of
+// the sum, rounded into R, would be lost where scores are large and alike (24 nodes at one distance of 1e9).
+//   Near zero (|R| below some 2^20) R = c, c = at unit rounded, and one multiply-add a score is exact up to the result's
+// own step.  Farther, at unit would be rounded by more than the exponents that matter: there R = at unit as it is, and
+// scores have `at` subtracted first, which is exact where they are close.  A wave takes that form for all its rows as
+// soon as one needs it; add = at unit - R says the same of the others.
+struct Around {
+    float at, c;
+    __device__ __forceinline__ bool far(float limit) const { return fabsf(c) >= limit && fabsf(at) < INFINITY; }
+    __device__ __forceinline__ float add(float unit, float limit) const {
+        return fabsf(c) < limit ? __builtin_fmaf(at, unit, -c) : 0.0f;
+    }
 };
-template <bool DIST, bool CAP>
-__device__ __forceinline__ Bias bias_of(const Args& a, float slope) {
-    Bias b;
-    b.plain = !CAP && a.scale > 1e-18f;
-    if (DIST) b.plain = b.plain && __all(slope > 0.0f && slope < 1e18f);
-    b.pre = CAP ? a.scale / a.cap : b.plain ? 1.0f : a.scale;
-    b.slope = b.plain ? -slope / a.scale : -slope;
-    b.unit = b.plain ? a.scale * kLog2e : kLog2e;
-    return b;
-}
+__device__ __forceinline__ Around around(float at, float unit) { return {at, at * unit}; }
+constexpr float kFar = 1048576.0f;
+// In the backward passes R comes from lse, and near zero two-byte types take the weights around it for probabilities:
+// they sum to 1 within 2^-14 up to 2^10, below a 2^5th of such a type's own step.
+template <typename T>
+constexpr float kFarBack = sizeof(T) == 2 ? 1024.0f : kFar;
 // what is done to every score of a lane's column: n over its tiles, r over a tile's four rows
 #define TRX_EACH_SCORE _Pragma("unroll") for (int n = 0; n < kTiles; ++n) _Pragma("unroll") for (int r = 0; r < 4; ++r)
 // Scores capped: cap tanh(s * pre), and with SLACK the tanh's slope 1 - tanh^2.  float32 takes the library's tanh.  For
@@ -402,6 +419,15 @@ __device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kT
                 if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
             }
         }
+    }
+}
+// the products of a tile to scores: with the scale, or capped
+template <typename T, bool CAP, bool SLACK, int kTiles>
+__device__ __forceinline__ void scores(const Call& call, f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles]) {
+    if (CAP) {
+        cap_scores<T, kTiles, SLACK>(s, slack, call.unit.pre, call.a.cap);
+    } else if (call.unit.pre != 1.0f) {
+        TRX_EACH_SCORE s[n][r] *= call.unit.pre;
     }
 }
 template <int N>

@@ -48,7 +48,7 @@ AttentionCut cut_fwd(const trx_node_attention_args& a) {
 AttentionCut cut_bwd_q(const trx_node_attention_args& a) {
     const int64_t G = a.heads / a.kv_heads;
     return cut(std::min(a.max_queries, a.num_queries) * G, std::min(a.max_nodes, a.num_nodes),
-               a.num_queries * G, a.num_graphs, a.kv_heads, a.num_queries * a.heads * (a.channels + 3) * 4, wide_bwd(a), 256);
+               a.num_queries * G, a.num_graphs, a.kv_heads, a.num_queries * a.heads * (a.channels + 4) * 4, wide_bwd(a), 256);
 }
 AttentionCut cut_bwd_kv(const trx_node_attention_args& a) {
     const int64_t G = a.heads / a.kv_heads;
@@ -56,9 +56,10 @@ AttentionCut cut_bwd_kv(const trx_node_attention_args& a) {
                a.num_nodes, a.num_graphs, a.kv_heads, a.num_nodes * a.kv_heads * a.channels * 8, wide_bwd(a), 256);
 }
 
-// each row's <go, out> and slope gradient, the slope chunks' sums; the splits of one pass after the other follow
+// each row's <go, out>, inverse of its weights' sum and slope gradient, the slope chunks' sums; the splits of one pass
+// after the other follow
 size_t attention_row_floats(const trx_node_attention_args& a) {
-    return ((size_t)a.num_queries * a.heads * 2 + (size_t)kSlopeChunks * a.heads + 3) / 4 * 4;
+    return ((size_t)a.num_queries * a.heads * 3 + (size_t)kSlopeChunks * a.heads + 3) / 4 * 4;
 }
 
 size_t node_attention_workspace(const trx_node_attention_args& a, bool backward) {
@@ -67,7 +68,7 @@ size_t node_attention_workspace(const trx_node_attention_args& a, bool backward)
         return splits > 1 ? (size_t)splits * a.num_queries * a.heads * (a.channels + 2) * sizeof(float) : 0;
     }
     const int sq = cut_bwd_q(a).splits, skv = cut_bwd_kv(a).splits;
-    const size_t q = sq > 1 ? (size_t)sq * a.num_queries * a.heads * (a.channels + 3) : 0;
+    const size_t q = sq > 1 ? (size_t)sq * a.num_queries * a.heads * (a.channels + 4) : 0;
     const size_t kv = skv > 1 ? (size_t)skv * a.num_nodes * a.kv_heads * a.channels * 2 : 0;
     return (attention_row_floats(a) + std::max(q, kv)) * sizeof(float);
 }

@@ -1,6 +1,7 @@
 // node_attention_bwd.h -- node_attention's gradients, one element type to a
-// translation unit (node_attention_{f32,bf16,f16}.hip): with p the probabilities, brought back from the saved lse, go the incoming
-// gradient, gp = go v^T and D = <go, out> of each row,
+// translation unit (node_attention_{f32,bf16,f16}.hip): with p the probabilities,
+// brought back from the saved lse, go the incoming gradient, gp = go v^T and D =
+// <go, out> of each row,
 //   t = p (gp - D);  grad_slope = -sum t d;  u = t (1 - tanh^2)
 //   grad_q = scale u k;  grad_k = scale u^T q;  grad_v = p^T go.
 // Two passes and no atomics: one workgroup keeps query rows and runs over the
@@ -27,15 +28,24 @@
 namespace trx {
 namespace {
 
-// Per (query row, head): what the slope's gradient needs.  D is off by its own roundings, so sum t is not quite zero;
-// what is left of it corrects sum t d: grad_slope of the row = (sum t)(sum p d) - sum t d.
-struct SlopeSums {
-    float t, pd, td;
+// Per (query row, head), summed with weights around lse: their sum, which is 1 but for what rounding took from lse
+// and divides everything else, and what the slope's gradient needs.  D is off by its own roundings, so sum t is not
+// quite zero; what is left of it corrects sum t d: grad_slope of the row = (sum t)(sum p d) - sum t d.
+struct Sums {
+    float e, t, pd, td;
+    __device__ __forceinline__ float inverse() const { return e == 0.0f ? 0.0f : 1.0f / e; }
+    __device__ __forceinline__ float slope(float inv) const {
+        return __builtin_fmaf(t * inv, pd * inv, -(td * inv));
+    }
+};
+// where they go, for the pass over the keys and for the slopes' sums (slopes: NULL where not wanted)
+struct RowSums {
+    float *dots, *inverse, *slopes;
 };
 
 template <typename T, int CP, int MQ, int WAVES, int KT, bool DIST, bool CAP>
 __global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, CP, WAVES>)))
-attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
+attention_bwd_q_kernel(Call call, RowSums out, float* part) {
     constexpr int kThreads = kWave * WAVES, kRows = 16 * MQ * WAVES, kSteps = CP / 32, kTiles = KT / 16;
     constexpr bool kAhead = WAVES > 1;   // one wave's registers are better spent on more waves
     constexpr bool kStageD = DIST && WAVES > 1;
@@ -45,6 +55,7 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
     const int G = call.group.by, C = a.channels;
+    const float unit = call.unit.log2;
     T* grad_q = static_cast<T*>(a.grad_q);
     if ((int)blockIdx.x >= call.blocks) {
         if (!part) zero_rest(grad_q, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
@@ -73,10 +84,11 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
         if (kAhead && first < last) fetch(first);
         frag<T> q[MQ][kSteps], go[MQ][kSteps];
         const float* dist[MQ];
-        Bias bias[MQ];
-        float lse[MQ], D[MQ];
+        Around ref[MQ];
+        bool far[MQ];
+        float slope[MQ], D[MQ];
         int limit[MQ];
-        SlopeSums sums[MQ];
+        Sums sums[MQ];
         f32x4 acc[MQ][CP / 16];
 #pragma unroll
         for (int t = 0; t < MQ; ++t) {
@@ -102,15 +114,16 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
                 }
             }
             D[t] = column_sum(dot);
-            bias[t] = bias_of<DIST, CAP>(a, DIST && a.slope ? a.slope[h] : 0.0f);
+            slope[t] = DIST && a.slope ? -a.slope[h] : 0.0f;
             if (DIST && !kStageD) {
                 dist[t] = a.dist + b * a.dist_graph + i * a.dist_row;
                 limit[t] = i < a.dist_rows ? min(ks.n, a.dist_cols) : 0;
             }
-            lse[t] = a.lse[at];
-            if (lse[t] == -INFINITY) lse[t] = INFINITY;   // an empty row: every probability comes out as zero
-            if (split == 0 && g == 0 && row0 + 16 * t + c < rows) dots[at] = D[t];
-            sums[t] = {0.0f, 0.0f, 0.0f};
+            const float lse = a.lse[at];   // an empty row: every weight comes out as zero
+            ref[t] = around(lse == -INFINITY ? INFINITY : lse * call.unit.per, unit);
+            far[t] = __any(ref[t].far(kFarBack<T>));
+            if (split == 0 && g == 0 && row0 + 16 * t + c < rows) out.dots[at] = D[t];
+            sums[t] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) acc[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -167,34 +180,35 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
                     for (int n = 0; n < kTiles; ++n)
                         d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + d_row[t] + 16 * n + 4 * g);
                 }
-                const float slope = bias[t].slope, unit = bias[t].unit;
                 f32x4 slack[kTiles];
-                if (CAP) {
-                    cap_scores<T, kTiles, true>(s[t], slack, bias[t].pre, a.cap);
-                } else if (!bias[t].plain) {
-                    TRX_EACH_SCORE s[t][n][r] *= bias[t].pre;
-                }
+                scores<T, CAP, true>(call, s[t], slack);
                 if (DIST) {
                     // beside weights of zero a distance must not be infinite in the slopes' sums
-                    if (__all(slope < 0.0f) && ordinary(d[t])) {
-                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope, d[t][n][r], s[t][n][r]);
-                        if (slopes) TRX_EACH_SCORE d[t][n][r] = fminf(d[t][n][r], 3e38f);
+                    if (__all(slope[t] < 0.0f) && ordinary(d[t])) {
+                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope[t], d[t][n][r], s[t][n][r]);
+                        if (out.slopes) TRX_EACH_SCORE d[t][n][r] = fminf(d[t][n][r], 3.402823466e38f);
                     } else {
                         TRX_EACH_SCORE {
                             const bool seen = finite(d[t][n][r]);
-                            s[t][n][r] = seen ? __builtin_fmaf(slope, d[t][n][r], s[t][n][r]) : -INFINITY;
+                            s[t][n][r] = seen ? __builtin_fmaf(slope[t], d[t][n][r], s[t][n][r]) : -INFINITY;
                             d[t][n][r] = seen ? d[t][n][r] : 0.0f;
                         }
                     }
                 } else if (j0 + KT > last) {
                     TRX_EACH_SCORE if (j0 + 16 * n + 4 * g + r >= last) s[t][n][r] = -INFINITY;
                 }
-                TRX_EACH_SCORE {
-                    const float p = exp2_fast(__builtin_fmaf(s[t][n][r], unit, -lse[t]));
-                    s[t][n][r] = p;
-                    gp[t][n][r] = p * (gp[t][n][r] - D[t]);
+                float minus = -ref[t].c;
+                if (far[t]) {   // a weight is at most 1: a score rounded otherwise than in the forward must not pass it
+                    TRX_EACH_SCORE s[t][n][r] = fminf(s[t][n][r] - ref[t].at, 0.0f);
+                    minus = ref[t].add(unit, kFarBack<T>);
                 }
-                if (DIST && slopes) {
+                TRX_EACH_SCORE {
+                    const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, minus));
+                    s[t][n][r] = e;
+                    sums[t].e += e;
+                    gp[t][n][r] = e * (gp[t][n][r] - D[t]);
+                }
+                if (DIST && out.slopes) {
                     TRX_EACH_SCORE {
                         sums[t].t += gp[t][n][r];
                         sums[t].pd = __builtin_fmaf(s[t][n][r], d[t][n][r], sums[t].pd);
@@ -216,29 +230,62 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
 #pragma unroll
         for (int t = 0; t < MQ; ++t) {
             const int row = row0 + 16 * t + c;
-            const float st = column_sum(sums[t].t), spd = column_sum(sums[t].pd), std_ = column_sum(sums[t].td);
+            Sums sum{column_sum(sums[t].e), 0.0f, 0.0f, 0.0f};
+            if (DIST && out.slopes) {
+                sum.t = column_sum(sums[t].t);
+                sum.pd = column_sum(sums[t].pd);
+                sum.td = column_sum(sums[t].td);
+            }
             if (row >= rows) continue;
             const int i = call.group(row), h = hk * G + (row - i * G);
             const int64_t all = a.num_queries * a.heads, at = (qs.at + i) * a.heads + h;
             if (part) {
                 const int64_t mine = split * all + at;
-                float* stat = part + (int64_t)splits * all * C;
-                if (slopes && g == 0) {
-                    stat[3 * mine] = st;
-                    stat[3 * mine + 1] = spd;
-                    stat[3 * mine + 2] = std_;
-                }
+                if (g == 0) reinterpret_cast<Sums*>(part + (int64_t)splits * all * C)[mine] = sum;
 #pragma unroll
                 for (int x = 0; x < CP / 16; ++x)
                     if (16 * x + 4 * g < C) *reinterpret_cast<f32x4*>(part + mine * C + 16 * x + 4 * g) = acc[t][x];
             } else {
-                if (slopes && g == 0) slopes[at] = __builtin_fmaf(st, spd, -std_);
+                const float inv = sum.inverse();
+                if (g == 0) {
+                    out.inverse[at] = inv;
+                    if (out.slopes) out.slopes[at] = sum.slope(inv);
+                }
 #pragma unroll
                 for (int x = 0; x < CP / 16; ++x)
                     if (16 * x + 4 * g < C)
-                        put4(grad_q, static_cast<T*>(nullptr), at * C + 16 * x + 4 * g, acc[t][x] * a.scale);
+                        put4(grad_q, static_cast<T*>(nullptr), at * C + 16 * x + 4 * g, acc[t][x] * inv * a.scale);
             }
         }
+    }
+}
+
+// grad_q, its rows' sums and slope gradients from the splits'; rows of no graph zero: four channels a thread
+template <typename T>
+__global__ void __launch_bounds__(256) join_grad_q_kernel(Args a, RowSums out, const float* part, int splits) {
+    const Span qs = all_rows(a.q_ptr, a.num_graphs, a.num_queries);
+    const int C = a.channels, C4 = C / 4;
+    const int64_t all = a.num_queries * a.heads, step = (int64_t)gridDim.x * 256;
+    const Sums* sums = reinterpret_cast<const Sums*>(part + splits * all * C);
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all * C4; x += step) {
+        const int64_t at = x / C4, row = at / a.heads, e = x * 4;
+        f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+        if (row >= qs.at && row < qs.at + qs.n) {
+            Sums sum{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (int k = 0; k < splits; ++k) {
+                v = v + *reinterpret_cast<const f32x4*>(part + k * all * C + e);
+                const Sums s = sums[k * all + at];
+                sum = {sum.e + s.e, sum.t + s.t, sum.pd + s.pd, sum.td + s.td};
+            }
+            const float inv = sum.inverse();
+            v = v * inv;
+            if (x == at * C4) {
+                out.inverse[at] = inv;
+                if (out.slopes) out.slopes[at] = sum.slope(inv);
+            }
+        }
+        put4(static_cast<T*>(a.grad_q), static_cast<T*>(nullptr), e, v * a.scale);
     }
 }
 
@@ -246,14 +293,16 @@ attention_bwd_q_kernel(Call call, float* dots, float* slopes, float* part) {
 // in the other passes this one took 184 us at 4001 nodes; it took 157 us once that and some of its score code went.
 template <typename T, int CP, int MK, int WAVES, int RT, bool DIST, bool CAP>
 __global__ void __launch_bounds__(kWave* WAVES) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, CP, WAVES>)))
-attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
+attention_bwd_kv_kernel(Call call, const float* dots, const float* inverse, float* part) {
     constexpr int kThreads = kWave * WAVES, kKeys = 16 * MK * WAVES, kSteps = CP / 32, kTiles = RT / 16;
-    constexpr bool kAhead = WAVES > 1;
+    constexpr bool kAhead = WAVES > 1, kDivide = sizeof(T) == 4;   // kDivide: by the weights' sum, near zero too
     __shared__ __attribute__((aligned(16))) T q_tile[RT * kRow<T, CP>], go_tile[RT * kRow<T, CP>];
-    __shared__ __attribute__((aligned(16))) float row_lse[RT], row_D[RT], row_slope[RT];
+    __shared__ __attribute__((aligned(16))) float row_at[RT], row_minus[RT], row_inv[RT], row_D[RT], row_slope[RT];
+    __shared__ int tile_far;
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
     const int G = call.group.by, C = a.channels;
+    const float unit = call.unit.log2;
     T *grad_k = static_cast<T*>(a.grad_k), *grad_v = static_cast<T*>(a.grad_v);
     if ((int)blockIdx.x >= call.blocks) {
         if (part) return;
@@ -271,12 +320,9 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
         first = min((int64_t)rows, (int64_t)split * each);
         last = min((int64_t)rows, (int64_t)first + each);
     }
-    const bool plain = !CAP && a.scale > 1e-18f;
-    const float pre = CAP ? a.scale / a.cap : plain ? 1.0f : a.scale, unit = plain ? a.scale * kLog2e : kLog2e;
-    const float per = plain ? -1.0f / a.scale : -1.0f;
     bool falls = DIST && a.slope;   // all the group's slopes are positive
     if (falls)
-        for (int h = lane; h < G; h += kWave) falls = falls && a.slope[hk * G + h] > 0.0f && a.slope[hk * G + h] < 1e18f;
+        for (int h = lane; h < G; h += kWave) falls = falls && a.slope[hk * G + h] > 0.0f;
     falls = __all(falls);
 
     for (int tile = work.tile; (int64_t)tile * kKeys < ks.n; tile += call.tiles) {
@@ -306,7 +352,8 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
             for (int x = 0; x < CP / 16; ++x) gk[t][x] = gv[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         Staged<T, CP, RT, kThreads> q_next, go_next;
-        float next_lse = 0.0f, next_D = 0.0f, next_slope = 0.0f;
+        Around next{0.0f, 0.0f};
+        float next_inv = 0.0f, next_D = 0.0f, next_slope = 0.0f;
         auto fetch = [&](int r0) {
             q_next.load_rows(r0, rows, C, [&](int row) {
                 const int i = call.group(row), h = hk * G + (row - i * G);
@@ -316,17 +363,18 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                 const int i = call.group(row), h = hk * G + (row - i * G);
                 return static_cast<const T*>(a.grad_out) + ((qs.at + i) * a.heads + h) * C;
             });
-            next_lse = INFINITY;   // rows that are not there, and empty ones: every probability comes out as zero
-            next_D = 0.0f;
+            next = {INFINITY, INFINITY};   // rows that are not there, and empty ones: every weight comes out as zero
+            next_D = next_inv = 0.0f;
             next_slope = -1.0f;    // as any row's where all fall: with 0, a distance of +inf would make NaN
             if (threadIdx.x < RT && r0 + (int)threadIdx.x < last) {
                 const int row = r0 + threadIdx.x, i = call.group(row), h = hk * G + (row - i * G);
                 const int64_t at = (qs.at + i) * a.heads + h;
                 if (a.lse[at] != -INFINITY) {
-                    next_lse = a.lse[at];
+                    next = around(a.lse[at] * call.unit.per, unit);
+                    next_inv = inverse[at];
                     next_D = dots[at];
                 }
-                if (DIST) next_slope = a.slope ? a.slope[h] * per : 0.0f;
+                if (DIST) next_slope = a.slope ? -a.slope[h] : 0.0f;
             }
         };
         f32x4 d[MK][kTiles];
@@ -362,8 +410,14 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
             q_next.store(q_tile);
             go_next.store(go_tile);
             if (threadIdx.x < RT) {
-                row_lse[threadIdx.x] = next_lse;
+                const bool far = __any(next.far(kFarBack<T>));   // RT threads of the first wave
+                float minus = -next.c;
+                if (far) minus = next.add(unit, kFarBack<T>) + (kDivide ? 0.0f : log2f(next_inv));
+                row_at[threadIdx.x] = next.at;
+                row_minus[threadIdx.x] = minus;
+                if (kDivide) row_inv[threadIdx.x] = next_inv;
                 row_D[threadIdx.x] = next_D;
+                tile_far = far;
                 if (DIST) row_slope[threadIdx.x] = next_slope;
             }
             __syncthreads();
@@ -388,21 +442,19 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                 }
             }
             frag<T> p[MK][RT / 32], u[MK][RT / 32];
-            f32x4 lse[kTiles], D[kTiles], slope[kTiles];
+            const bool far = tile_far;
+            f32x4 minus[kTiles], inv[kTiles], D[kTiles], slope[kTiles];
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) {
-                lse[n] = *reinterpret_cast<const f32x4*>(row_lse + 16 * n + 4 * g);
+                minus[n] = *reinterpret_cast<const f32x4*>(row_minus + 16 * n + 4 * g);
+                if (kDivide) inv[n] = *reinterpret_cast<const f32x4*>(row_inv + 16 * n + 4 * g);
                 D[n] = *reinterpret_cast<const f32x4*>(row_D + 16 * n + 4 * g);
                 if (DIST) slope[n] = *reinterpret_cast<const f32x4*>(row_slope + 16 * n + 4 * g);
             }
 #pragma unroll
             for (int t = 0; t < MK; ++t) {
                 f32x4 slack[kTiles];
-                if (CAP) {
-                    cap_scores<T, kTiles, true>(s[t], slack, pre, a.cap);
-                } else if (!plain) {
-                    TRX_EACH_SCORE s[t][n][r] *= pre;
-                }
+                scores<T, CAP, true>(call, s[t], slack);
                 if (DIST) {
                     if (falls && ordinary(d[t])) {
                         TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope[n][r], d[t][n][r], s[t][n][r]);
@@ -411,8 +463,12 @@ attention_bwd_kv_kernel(Call call, const float* dots, float* part) {
                             finite(d[t][n][r]) ? __builtin_fmaf(slope[n][r], d[t][n][r], s[t][n][r]) : -INFINITY;
                     }
                 }
+                if (far) {
+                    TRX_EACH_SCORE s[t][n][r] = fminf(s[t][n][r] - row_at[16 * n + 4 * g + r], 0.0f);
+                }
                 TRX_EACH_SCORE {   // both rounded to the type for their products
-                    const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, -lse[n][r]));
+                    float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, minus[n][r]));
+                    if (kDivide) e *= inv[n][r];
                     const float v = e * (gp[t][n][r] - D[n][r]);
                     p[t][n / 2][4 * (n % 2) + r] = (T)e;
                     u[t][n / 2][4 * (n % 2) + r] = (T)(CAP ? v * slack[n][r] : v);
@@ -476,8 +532,8 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(SplitSum first, SplitSu
     }
 }
 
-// A (head, chunk of the query rows) each: the sum of the rows' slope gradients, from `slopes`, or from the splits'
-// sums in `stat` where there are any; chunk by chunk to out[head + heads * chunk].  A fixed order throughout.
+// A (head, chunk of the query rows) each: the sum of the rows' slope gradients; chunk by chunk to out[head + heads *
+// chunk].  A fixed order throughout.
 template <int kBlock>
 __device__ __forceinline__ float block_sum(float v) {
     __shared__ float part[kBlock / kWave];
@@ -492,27 +548,14 @@ __device__ __forceinline__ float block_sum(float v) {
 }
 template <typename T>
 __global__ void __launch_bounds__(1024)
-    slope_rows_kernel(Args a, const float* slopes, const float* stat, int splits, float* out) {
+    slope_rows_kernel(Args a, const float* slopes, float* out) {
     const int h = blockIdx.x;
-    const int64_t all = a.num_queries * a.heads, each = (a.num_queries + gridDim.y - 1) / gridDim.y;
+    const int64_t each = (a.num_queries + gridDim.y - 1) / gridDim.y;
     const Span s = all_rows(a.q_ptr, a.num_graphs, a.num_queries);
     const int64_t begin = max(s.at, (int64_t)blockIdx.y * each), end = min(s.at + s.n, (int64_t)(blockIdx.y + 1) * each);
     float v = 0.0f;
 #pragma unroll 4
-    for (int64_t r = begin + threadIdx.x; r < end; r += 1024) {
-        const int64_t at = r * a.heads + h;
-        if (stat) {
-            float t = 0.0f, pd = 0.0f, td = 0.0f;
-            for (int k = 0; k < splits; ++k) {
-                t += stat[3 * (k * all + at)];
-                pd += stat[3 * (k * all + at) + 1];
-                td += stat[3 * (k * all + at) + 2];
-            }
-            v += __builtin_fmaf(t, pd, -td);
-        } else {
-            v += slopes[at];
-        }
-    }
+    for (int64_t r = begin + threadIdx.x; r < end; r += 1024) v += slopes[r * a.heads + h];
     v = block_sum<1024>(v);
     if (threadIdx.x == 0) out[blockIdx.y * a.heads + h] = v;
 }
@@ -524,9 +567,11 @@ __global__ void __launch_bounds__(kWave) slope_chunks_kernel(const float* chunks
 
 template <typename T, int CP, bool DIST, bool CAP>
 void launch_bwd(const Args& a, hipStream_t stream) {
-    float *dots = static_cast<float*>(a.workspace), *slopes = dots + a.num_queries * a.heads;
-    float *chunks = slopes + a.num_queries * a.heads, *split = dots + attention_row_floats(a);
+    const int64_t rows = a.num_queries * a.heads;
+    float *dots = static_cast<float*>(a.workspace), *inverse = dots + rows, *slopes = inverse + rows;
+    float *chunks = slopes + rows, *split = dots + attention_row_floats(a);
     const bool want_slopes = DIST && a.grad_slope && a.slope;
+    const RowSums sums{dots, inverse, want_slopes ? slopes : nullptr};
     auto blocks = [](int64_t n) { return (unsigned)std::min<int64_t>(2048, (n / 4 + 255) / 256); };
     // 128 channels: of 32 rows a wave, operands, accumulators and both score tiles leave no registers to load ahead
     constexpr int M = kTilesOfWave<T, CP>, MQ = CP == 128 ? 1 : 2, MK = CP == 128 ? 1 : 2;
@@ -536,26 +581,24 @@ void launch_bwd(const Args& a, hipStream_t stream) {
         const Call call = call_of(a, c);
         const dim3 grid(call.blocks + kRestBlocks);
         if (c.narrow)
-            hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, M, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
-                               want_slopes ? slopes : nullptr, part);
+            hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, M, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, sums,
+                               part);
         else
-            hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, MQ, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call, dots,
-                               want_slopes ? slopes : nullptr, part);
+            hipLaunchKernelGGL((attention_bwd_q_kernel<T, CP, MQ, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call, sums,
+                               part);
         const int64_t n = a.num_queries * a.heads * a.channels;
         if (part)
-            hipLaunchKernelGGL(sum_splits_kernel<T>, dim3(blocks(n)), dim3(256), 0, stream,
-                               SplitSum{part, a.grad_q, a.scale}, SplitSum{}, c.splits, n, n,
-                               (int64_t)a.heads * a.channels, a.q_ptr, a.num_graphs, a.num_queries);
+            hipLaunchKernelGGL(join_grad_q_kernel<T>, dim3(blocks(n)), dim3(256), 0, stream, a, sums, part, c.splits);
         if (want_slopes) {
             const int count = (int)std::max<int64_t>(1, std::min<int64_t>(kSlopeChunks, a.num_queries / 16384));
             hipLaunchKernelGGL(slope_rows_kernel<T>, dim3(a.heads, count), dim3(1024), 0, stream, a, slopes,
-                               part ? part + c.splits * n : nullptr, c.splits, count > 1 ? chunks : a.grad_slope);
+                               count > 1 ? chunks : a.grad_slope);
             if (count > 1)
                 hipLaunchKernelGGL(slope_chunks_kernel<T>, dim3(a.heads), dim3(kWave), 0, stream, chunks, count, a.heads,
                                    a.grad_slope);
         }
     } else if (want_slopes) {
-        hipLaunchKernelGGL(slope_rows_kernel<T>, dim3(a.heads), dim3(1024), 0, stream, a, slopes, nullptr, 1, a.grad_slope);
+        hipLaunchKernelGGL(slope_rows_kernel<T>, dim3(a.heads), dim3(1024), 0, stream, a, slopes, a.grad_slope);
     }
     if (a.num_nodes > 0) {
         const AttentionCut c = cut_bwd_kv(a);
@@ -564,10 +607,10 @@ void launch_bwd(const Args& a, hipStream_t stream) {
         const dim3 grid(call.blocks + kRestBlocks);
         if (c.narrow)
             hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, MK, 1, 32, DIST, CAP>), grid, dim3(64), 0, stream, call, dots,
-                               part);
+                               inverse, part);
         else
             hipLaunchKernelGGL((attention_bwd_kv_kernel<T, CP, MK, 4, 32, DIST, CAP>), grid, dim3(256), 0, stream, call,
-                               dots, part);
+                               dots, inverse, part);
         if (part) {
             const int64_t n = a.num_nodes * a.kv_heads * a.channels;
             hipLaunchKernelGGL(sum_splits_kernel<T>, dim3(blocks(n), 2), dim3(256), 0, stream,

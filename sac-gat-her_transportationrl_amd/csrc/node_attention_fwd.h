@@ -37,6 +37,7 @@ attention_fwd_kernel(Call call, float* part) {
     const Args& a = call.a;
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane / 16, c = lane % 16;
     const int G = call.group.by, C = a.channels;
+    const float unit = call.unit.log2;
     T* out = static_cast<T*>(a.out);
     if ((int)blockIdx.x >= call.blocks) {
         if (!part) zero_rest(out, a.q_ptr, a.num_graphs, a.num_queries, (int64_t)a.heads * C, blockIdx.x - call.blocks);
@@ -65,8 +66,9 @@ attention_fwd_kernel(Call call, float* part) {
         if (kAhead && first < last) fetch(first);
         frag<T> q[MQ][kSteps];
         const float* dist[MQ];
-        Bias bias[MQ];
-        float m[MQ], l[MQ];   // the reference point in units of log 2, the sum
+        Around ref[MQ];
+        float m[MQ], l[MQ], slope[MQ];   // the reference's score (-inf: none yet), the sum, -slope
+        bool far[MQ];                    // of the wave
         int limit[MQ];
         f32x4 o[MQ][CP / 16];
 #pragma unroll
@@ -76,12 +78,14 @@ attention_fwd_kernel(Call call, float* part) {
             const T* p = static_cast<const T*>(a.q) + (qs.at + i) * a.q_row + h * a.q_head;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) q[t][s] = 32 * s + 8 * g < C ? load_frag(p + 32 * s + 8 * g) : zero_frag<T>();
-            bias[t] = bias_of<DIST, CAP>(a, DIST && a.slope ? a.slope[h] : 0.0f);
+            slope[t] = DIST && a.slope ? -a.slope[h] : 0.0f;
             if (DIST && !kStageD) {
                 dist[t] = a.dist + b * a.dist_graph + i * a.dist_row;
                 limit[t] = i < a.dist_rows ? min(ks.n, a.dist_cols) : 0;
             }
             m[t] = -INFINITY;
+            ref[t] = {0.0f, 0.0f};
+            far[t] = false;
             l[t] = 0.0f;
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) o[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -133,39 +137,43 @@ attention_fwd_kernel(Call call, float* part) {
                     for (int n = 0; n < kTiles; ++n)
                         d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + d_row[t] + 16 * n + 4 * g);
                 }
-                // scores in bias.unit, and their maximum
-                if (CAP) {
-                    cap_scores<T, kTiles, false>(s[t], s[t], bias[t].pre, a.cap);
-                } else if (!bias[t].plain) {
-                    TRX_EACH_SCORE s[t][n][r] *= bias[t].pre;
-                }
+                scores<T, CAP, false>(call, s[t], s[t]);
                 if (DIST) {
-                    const float slope = bias[t].slope;
-                    if (__all(slope < 0.0f) && ordinary(d[t])) {
-                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope, d[t][n][r], s[t][n][r]);
+                    if (__all(slope[t] < 0.0f) && ordinary(d[t])) {   // a distance of +inf makes its -inf by itself
+                        TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope[t], d[t][n][r], s[t][n][r]);
                     } else {
                         TRX_EACH_SCORE s[t][n][r] =
-                            finite(d[t][n][r]) ? __builtin_fmaf(slope, d[t][n][r], s[t][n][r]) : -INFINITY;
+                            finite(d[t][n][r]) ? __builtin_fmaf(slope[t], d[t][n][r], s[t][n][r]) : -INFINITY;
                     }
                 } else if (j0 + KT > last) {
                     TRX_EACH_SCORE if (j0 + 16 * n + 4 * g + r >= last) s[t][n][r] = -INFINITY;
                 }
                 float top = -INFINITY;
                 TRX_EACH_SCORE top = fmaxf(top, s[t][n][r]);
-                top = column_max(top) * bias[t].unit;
+                top = column_max(top);
                 // The reference point moves only when a score passes it by 2^8: nothing is lost in float32, and the
                 // accumulators are rescaled once or twice a row instead of at every new maximum.
-                const bool move = top > m[t] + 8.0f;
+                const bool move = (top - m[t]) * unit > 8.0f;
                 if (__any(move)) {
-                    const float f = move ? exp2_fast(m[t] - top) : 1.0f;
-                    m[t] = move ? top : m[t];
+                    const Around next = around(top, unit);
+                    const float by = next.add(unit, kFar) - ref[t].add(unit, kFar);
+                    const float f = move ? exp2_fast(__builtin_fmaf(m[t] - top, unit, by)) : 1.0f;
+                    if (move) {
+                        m[t] = top;
+                        ref[t] = next;
+                    }
+                    far[t] = __any(ref[t].far(kFar));
                     l[t] *= f;
 #pragma unroll
                     for (int x = 0; x < CP / 16; ++x) o[t][x] = o[t][x] * f;
                 }
-                const float base = m[t] == -INFINITY ? 0.0f : -m[t], unit = bias[t].unit;
+                float minus = -ref[t].c;
+                if (far[t]) {
+                    TRX_EACH_SCORE s[t][n][r] -= ref[t].at;
+                    minus = ref[t].add(unit, kFar);
+                }
                 TRX_EACH_SCORE {
-                    const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, base));
+                    const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, minus));
                     l[t] += e;
                     p[t][n / 2][4 * (n % 2) + r] = (T)e;   // rounded to the type for the product with v
                 }
@@ -186,19 +194,22 @@ attention_fwd_kernel(Call call, float* part) {
             if (row >= rows) continue;
             const int i = call.group(row), h = hk * G + (row - i * G);
             const int64_t at = (qs.at + i) * a.heads + h;
-            if (part) {   // this split's sum and accumulator, for attention_join_kernel
+            const float add = ref[t].add(unit, kFar);   // 0 where m is still -inf
+            if (part) {   // this split's sum and accumulator around m unit, for the joining kernels
                 const int64_t all = a.num_queries * a.heads, mine = split * all + at;
                 float* stat = part + (int64_t)splits * all * C;
+                const float f = exp2_fast(-add);
                 if (g == 0) {
                     stat[2 * mine] = m[t];
-                    stat[2 * mine + 1] = sum;
+                    stat[2 * mine + 1] = sum * f;
                 }
 #pragma unroll
                 for (int x = 0; x < CP / 16; ++x)
-                    if (16 * x + 4 * g < C) *reinterpret_cast<f32x4*>(part + mine * C + 16 * x + 4 * g) = o[t][x];
+                    if (16 * x + 4 * g < C) *reinterpret_cast<f32x4*>(part + mine * C + 16 * x + 4 * g) = o[t][x] * f;
             } else {
                 const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (a.lse && g == 0) a.lse[at] = sum == 0.0f ? -INFINITY : m[t] + log2f(sum);
+                if (a.lse && g == 0)
+                    a.lse[at] = sum == 0.0f ? -INFINITY : __builtin_fmaf(log2f(sum) - add, kLn2, m[t] * call.unit.nat);
 #pragma unroll
                 for (int x = 0; x < CP / 16; ++x)
                     if (16 * x + 4 * g < C) put4(out, static_cast<T*>(a.out_low), at * C + 16 * x + 4 * g, o[t][x] * f);
@@ -209,7 +220,7 @@ attention_fwd_kernel(Call call, float* part) {
 
 // out, out_low and lse from few splits' sums, rows of no graph zero: four channels a thread
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join_few_kernel(Args a, const float* part, int splits) {
+__global__ void __launch_bounds__(256) attention_join_few_kernel(Args a, Unit unit, const float* part, int splits) {
     const Span qs = all_rows(a.q_ptr, a.num_graphs, a.num_queries);
     const int C = a.channels, C4 = C / 4;
     const int64_t all = a.num_queries * a.heads, step = (int64_t)gridDim.x * 256;
@@ -226,19 +237,19 @@ __global__ void __launch_bounds__(256) attention_join_few_kernel(Args a, const f
         for (int s = 0; s < splits; ++s) {
             const float m = stat[2 * (s * all + at)], l = stat[2 * (s * all + at) + 1];
             // a split without a finite score adds its sum as it is: zero, or the NaN that it saw
-            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+            const float f = m == -INFINITY ? 0.0f : exp2_fast((m - top) * unit.log2);
             sum += m == -INFINITY ? l : l * f;
             v = v + *reinterpret_cast<const f32x4*>(part + s * all * C + e) * f;
         }
         put4(static_cast<T*>(a.out), static_cast<T*>(a.out_low), e, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
-        if (a.lse && x == at * C4) a.lse[at] = sum == 0.0f ? -INFINITY : top + log2f(sum);
+        if (a.lse && x == at * C4) a.lse[at] = sum == 0.0f ? -INFINITY : __builtin_fmaf(log2f(sum), kLn2, top * unit.nat);
     }
 }
 
 // The same from many: a workgroup to a (row, head), its four waves
 // each over every fourth split, two channels a lane
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join_kernel(Args a, const float* part, int splits) {
+__global__ void __launch_bounds__(256) attention_join_kernel(Args a, Unit unit, const float* part, int splits) {
     __shared__ float sums[4][2 * kWave];
     const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, C = a.channels;
     const int64_t all = a.num_queries * a.heads, at = blockIdx.x;
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Args a, const float
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     // a split without a finite score adds its sum as it is: zero, or the NaN that it saw
-    const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
+    const float f = m == -INFINITY ? 0.0f : exp2_fast((m - top) * unit.log2);
     float sum = m == -INFINITY ? l : l * f;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -278,7 +289,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(Args a, const float
         static_cast<T*>(a.out)[at * C + ch] = t;
         if (a.out_low) static_cast<T*>(a.out_low)[at * C + ch] = (T)(v - (float)t);
     }
-    if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.0f ? -INFINITY : top + log2f(sum);
+    if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.0f ? -INFINITY : __builtin_fmaf(log2f(sum), kLn2, top * unit.nat);
 }
 
 template <typename T, int CP, bool DIST, bool CAP>
@@ -298,10 +309,10 @@ void launch_fwd(const Args& a, hipStream_t stream) {
     if (part && c.splits <= 8)
         hipLaunchKernelGGL(attention_join_few_kernel<T>,
                            dim3((unsigned)std::min<int64_t>(4096, (a.num_queries * a.heads * a.channels / 4 + 255) / 256)),
-                           dim3(256), 0, stream, a, part, c.splits);
+                           dim3(256), 0, stream, a, call.unit, part, c.splits);
     else if (part)
         hipLaunchKernelGGL(attention_join_kernel<T>, dim3((unsigned)(a.num_queries * a.heads)), dim3(256), 0, stream, a,
-                           part, c.splits);
+                           call.unit, part, c.splits);
 }
 
 }  // namespace
