@@ -360,15 +360,45 @@ __device__ __forceinline__ float column_max(float v) {
 // own step.  Farther, at unit would be rounded by more than the exponents that matter: there R = at unit as it is, and
 // scores have `at` subtracted first, which is exact where they are close.  A wave takes that form for all its rows as
 // soon as one needs it; add = at unit - R says the same of the others.
+//   `lift` puts R that far below at unit.
 struct Around {
     float at, c;
     __device__ __forceinline__ bool far(float limit) const { return fabsf(c) >= limit && fabsf(at) < INFINITY; }
-    __device__ __forceinline__ float add(float unit, float limit) const {
-        return fabsf(c) < limit ? __builtin_fmaf(at, unit, -c) : 0.0f;
+    __device__ __forceinline__ float add(float unit, float limit, float lift = 0.0f) const {
+        return fabsf(c) < limit ? __builtin_fmaf(at, unit, -c) : lift;
     }
 };
-__device__ __forceinline__ Around around(float at, float unit) { return {at, at * unit}; }
+__device__ __forceinline__ Around around(float at, float unit, float lift = 0.0f) {
+    return {at, __builtin_fmaf(at, unit, -lift)};
+}
 constexpr float kFar = 1048576.0f;
+// float16 ends at 2^16 and loses bits below 2^-14, so what is rounded to it is brought into that range first.
+// Forward: weights are 2^7 at the reference and at most 2^15; without, those below 2^-14 of the largest lose bits and
+// those below 2^-25 of it vanish from the product though the sum has them.  A probability in grad_v: by 2^15.
+template <typename T>
+constexpr bool kHalf = std::is_same_v<T, _Float16>;
+template <typename T>
+constexpr float kLift = kHalf<T> ? 7.0f : 0.0f;
+template <typename T>
+constexpr float kWeight = kHalf<T> ? 32768.0f : 1.0f;
+// A score's gradient has no scale that is known beforehand (it is as large as the incoming gradient over the nodes):
+// each column keeps a power of two that brings its largest so far to 2^8 .. 2^14, and its accumulators follow when one
+// passes that.  Nothing of it is left in the result.  (bfloat16 has float32's range and needs none of this.)
+struct Raise {
+    float by;
+    template <int N>
+    __device__ __forceinline__ void over(float most, f32x4 (&acc)[N]) {
+        if (__any(!(most * by <= 16384.0f))) {
+            const float top = column_max(most);
+            const float next =
+                top * by > 16384.0f ? __uint_as_float((262u - (__float_as_uint(top) >> 23)) << 23) : by;   // 2^8 / top
+#pragma unroll
+            for (int x = 0; x < N; ++x) acc[x] = acc[x] * (next / by);
+            by = next;
+        }
+    }
+};
+constexpr float kRaiseAll = 0x1p100f;   // until something has been seen
 // In the backward passes R comes from lse, and near zero two-byte types take the weights around it for probabilities:
 // they sum to 1 within 2^-14 up to 2^10, below a 2^5th of such a type's own step.
 template <typename T>

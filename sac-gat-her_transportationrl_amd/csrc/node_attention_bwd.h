@@ -90,6 +90,7 @@ attention_bwd_q_kernel(Call call, RowSums out, float* part) {
         int limit[MQ];
         Sums sums[MQ];
         f32x4 acc[MQ][CP / 16];
+        Raise raise[MQ];
 #pragma unroll
         for (int t = 0; t < MQ; ++t) {
             const int row = min(row0 + 16 * t + c, rows - 1);
@@ -124,6 +125,7 @@ attention_bwd_q_kernel(Call call, RowSums out, float* part) {
             far[t] = __any(ref[t].far(kFarBack<T>));
             if (split == 0 && g == 0 && row0 + 16 * t + c < rows) out.dots[at] = D[t];
             sums[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+            raise[t] = {kRaiseAll};
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) acc[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -216,7 +218,14 @@ attention_bwd_q_kernel(Call call, RowSums out, float* part) {
                     }
                 }
                 // rounded to the type for the product with k
-                TRX_EACH_SCORE u[t][n / 2][4 * (n % 2) + r] = (T)(CAP ? gp[t][n][r] * slack[n][r] : gp[t][n][r]);
+                if (CAP) TRX_EACH_SCORE gp[t][n][r] *= slack[n][r];
+                if constexpr (kHalf<T>) {
+                    float most = 0.0f;
+                    TRX_EACH_SCORE most = fmaxf(most, fabsf(gp[t][n][r]));
+                    raise[t].over(most, acc[t]);
+                    TRX_EACH_SCORE gp[t][n][r] *= raise[t].by;
+                }
+                TRX_EACH_SCORE u[t][n / 2][4 * (n % 2) + r] = (T)gp[t][n][r];
             }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x)
@@ -239,6 +248,10 @@ attention_bwd_q_kernel(Call call, RowSums out, float* part) {
             if (row >= rows) continue;
             const int i = call.group(row), h = hk * G + (row - i * G);
             const int64_t all = a.num_queries * a.heads, at = (qs.at + i) * a.heads + h;
+            if constexpr (kHalf<T>) {
+#pragma unroll
+                for (int x = 0; x < CP / 16; ++x) acc[t][x] = acc[t][x] * (1.0f / raise[t].by);
+            }
             if (part) {
                 const int64_t mine = split * all + at;
                 if (g == 0) reinterpret_cast<Sums*>(part + (int64_t)splits * all * C)[mine] = sum;
@@ -333,6 +346,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, const float* inverse, floa
         // (16 n + 4 g + r) / G = 16 n / G + 4 g / G + r / G for every power of two up to 16; r0 is a multiple of 32
         const bool steps = DIST && WAVES > 1 && 16 % G == 0 && a.dist_row < (1 << 22) && a.dist_cols >= ks.n;
         f32x4 gk[MK][CP / 16], gv[MK][CP / 16];
+        Raise raise[MK];
 #pragma unroll
         for (int t = 0; t < MK; ++t) {
             const int j = min(key0 + 16 * t + c, ks.n - 1);
@@ -350,6 +364,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, const float* inverse, floa
             }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) gk[t][x] = gv[t][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            raise[t] = {kRaiseAll};
         }
         Staged<T, CP, RT, kThreads> q_next, go_next;
         Around next{0.0f, 0.0f};
@@ -470,9 +485,16 @@ attention_bwd_kv_kernel(Call call, const float* dots, const float* inverse, floa
                     float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, minus[n][r]));
                     if (kDivide) e *= inv[n][r];
                     const float v = e * (gp[t][n][r] - D[n][r]);
-                    p[t][n / 2][4 * (n % 2) + r] = (T)e;
-                    u[t][n / 2][4 * (n % 2) + r] = (T)(CAP ? v * slack[n][r] : v);
+                    p[t][n / 2][4 * (n % 2) + r] = (T)(e * kWeight<T>);
+                    s[t][n][r] = CAP ? v * slack[n][r] : v;
                 }
+                if constexpr (kHalf<T>) {
+                    float most = 0.0f;
+                    TRX_EACH_SCORE most = fmaxf(most, fabsf(s[t][n][r]));
+                    raise[t].over(most, gk[t]);
+                    TRX_EACH_SCORE s[t][n][r] *= raise[t].by;
+                }
+                TRX_EACH_SCORE u[t][n / 2][4 * (n % 2) + r] = (T)s[t][n][r];
             }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x)
@@ -491,6 +513,13 @@ attention_bwd_kv_kernel(Call call, const float* dots, const float* inverse, floa
             const int j = key0 + 16 * t + c;
             if (j >= ks.n) continue;
             const int64_t all = a.num_nodes * a.kv_heads, at = (ks.at + j) * a.kv_heads + hk;
+            if constexpr (kHalf<T>) {
+#pragma unroll
+                for (int x = 0; x < CP / 16; ++x) {
+                    gk[t][x] = gk[t][x] * (1.0f / raise[t].by);
+                    gv[t][x] = gv[t][x] * (1.0f / kWeight<T>);
+                }
+            }
 #pragma unroll
             for (int x = 0; x < CP / 16; ++x) {
                 const int ch = 16 * x + 4 * g;

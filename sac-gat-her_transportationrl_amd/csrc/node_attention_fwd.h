@@ -155,8 +155,8 @@ attention_fwd_kernel(Call call, float* part) {
                 // accumulators are rescaled once or twice a row instead of at every new maximum.
                 const bool move = (top - m[t]) * unit > 8.0f;
                 if (__any(move)) {
-                    const Around next = around(top, unit);
-                    const float by = next.add(unit, kFar) - ref[t].add(unit, kFar);
+                    const Around next = around(top, unit, kLift<T>);
+                    const float by = next.add(unit, kFar, kLift<T>) - ref[t].add(unit, kFar, kLift<T>);
                     const float f = move ? exp2_fast(__builtin_fmaf(m[t] - top, unit, by)) : 1.0f;
                     if (move) {
                         m[t] = top;
@@ -170,7 +170,7 @@ attention_fwd_kernel(Call call, float* part) {
                 float minus = -ref[t].c;
                 if (far[t]) {
                     TRX_EACH_SCORE s[t][n][r] -= ref[t].at;
-                    minus = ref[t].add(unit, kFar);
+                    minus = ref[t].add(unit, kFar, kLift<T>);
                 }
                 TRX_EACH_SCORE {
                     const float e = exp2_fast(__builtin_fmaf(s[t][n][r], unit, minus));
@@ -194,7 +194,7 @@ attention_fwd_kernel(Call call, float* part) {
             if (row >= rows) continue;
             const int i = call.group(row), h = hk * G + (row - i * G);
             const int64_t at = (qs.at + i) * a.heads + h;
-            const float add = ref[t].add(unit, kFar);   // 0 where m is still -inf
+            const float add = ref[t].add(unit, kFar, kLift<T>);   // 0 where m is still -inf
             if (part) {   // this split's sum and accumulator around m unit, for the joining kernels
                 const int64_t all = a.num_queries * a.heads, mine = split * all + at;
                 float* stat = part + (int64_t)splits * all * C;
