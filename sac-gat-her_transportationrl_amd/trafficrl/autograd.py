@@ -2,6 +2,15 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
+
+
+def no_tangents(what: str, *tensors) -> None:
+    """RuntimeError where a tensor (None: skipped) carries a forward-mode tangent,
+    which kernels called past autograd would drop without a word."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 class _NoSecond(torch.autograd.Function):

@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ..autograd import once
+from ..autograd import no_tangents, once
 
 
 def _strided(t: torch.Tensor) -> torch.Tensor:
@@ -114,11 +114,11 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
     rows; hints that shape the launch.  Give them where a batch holds many
     small networks: without, it takes several times as long.
 
-    Differentiable once in q, k, v and slope.  Scores, softmax statistics and
-    sums are float32; with half types the probabilities and the scores'
-    gradients are rounded to the type where they enter a matrix product.
-    Results do not depend on timing: no float atomics.  Asynchronous on the
-    current stream and capturable; before a backward pass is captured, drop
+    Differentiable once in q, k, v and slope (a forward-mode tangent is refused).
+    Scores, softmax statistics and sums are float32; with half types the
+    probabilities and the scores' gradients are rounded to the type where they
+    enter a matrix product.  Results do not depend on timing: no float atomics.
+    Asynchronous on the current stream and capturable; before a backward pass is captured, drop
     the eager graphs of the same leaves (autograd ties a leaf's accumulation to
     the stream of its first live graph)."""
     what = "node_attention"
@@ -165,6 +165,7 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
     max_nodes = nodes if max_nodes is None else int(max_nodes)
     if max_queries < 0 or max_nodes < 0:
         raise ValueError(f"{what}: max_queries and max_nodes must be >= 0")
+    no_tangents(what, q, k, v, dist, slope)
     _lib.same_device(what, q, k, v, ptr, k_ptr, dist, slope)
     q, k, v, ptr, k_ptr = _strided(q), _strided(k), _strided(v), ptr.contiguous(), k_ptr.contiguous()
     if dist is not None and dist.stride(-1) != 1:

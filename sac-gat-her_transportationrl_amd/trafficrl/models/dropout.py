@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ..autograd import once
+from ..autograd import no_tangents, once
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -69,8 +69,8 @@ def dropout_add(x: torch.Tensor, rng: torch.Tensor, p: float, *, residual: Optio
     Element e (row-major) is kept where its 16 bits of Philox4x32-10 reach
     round(65536 p); a dropped element adds nothing, whatever it holds.
 
-    Differentiable once in x and residual; the pair in use is kept with the
-    graph, so rng may move on before the backward pass.  Computed in float32,
+    Differentiable once in x and residual (a forward-mode tangent is refused);
+    the pair in use is kept with the graph, so rng may move on before the backward pass.  Computed in float32,
     rounded once.  Asynchronous on the current stream and capturable; before a
     backward pass is captured, drop the eager graphs of the same leaves."""
     what = "dropout_add"
@@ -84,6 +84,7 @@ def dropout_add(x: torch.Tensor, rng: torch.Tensor, p: float, *, residual: Optio
         raise ValueError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} for x {tuple(x.shape)} {x.dtype}")
     if not 0 <= int(site) < 2 ** 32:
         raise ValueError(f"{what}: site must be 0 .. 2^32 - 1, got {site}")
+    no_tangents(what, x, residual)
     _lib.same_device(what, x, rng, residual)
     x, rng, rest = _aligned(x), rng.contiguous(), (border, int(site), code)
     if residual is not None:

@@ -8,7 +8,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ..autograd import once
+from ..autograd import no_tangents, once
 
 
 _MASK_TYPES = (torch.float32, torch.bool, torch.uint8)
@@ -100,8 +100,8 @@ def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Option
     top_k links may be chosen the rest is -inf and -1.  A row with a logit of NaN
     or +inf that may be chosen has NaN for its values.
 
-    Differentiable once in logits through log_prob, entropy and top_log_prob.
-    Computed in float32 (the gradient rounded once to the logits' type).
+    Differentiable once in logits through log_prob, entropy and top_log_prob (a
+    forward-mode tangent is refused).  Computed in float32 (the gradient rounded once to the logits' type).
     Asynchronous on the current stream and capturable; before a backward pass is
     captured, drop the eager graphs of the same leaves."""
     what = "action_log_probs"
@@ -126,6 +126,7 @@ def action_log_probs(logits: torch.Tensor, action: torch.Tensor, *, mask: Option
     if max_row < 0:
         raise ValueError(f"{what}: max_row must be >= 0")
     max_row = min(max_row, 2 ** 30)
+    no_tangents(what, logits, mask)
     _lib.same_device(what, logits, action, mask, row_ptr)
     if logits.stride(-1) != 1 and logits.numel():
         logits = logits.contiguous()

@@ -122,3 +122,26 @@ def test_nodes_below_the_kernels_counters(nodes, code):
     assert L.trx_node_attention_workspace_bytes(a, 0) == -1
     a.num_nodes = a.max_nodes = (1 << 31) - (1 << 16)
     assert L.trx_node_attention_workspace_bytes(a, 1) > 0
+
+
+def test_tangents_are_refused():
+    """Forward-mode inputs that need no gradient would come back as constants."""
+    from torch.autograd import forward_ad
+    from trafficrl.models import dropout_add, node_attention
+    from trafficrl.rl import action_log_probs
+    p, rng = torch.tensor([0, 6]), torch.tensor([1, 2])
+    x, logits = torch.randn(6, 2, 32), torch.randn(4, 9)
+    act = torch.zeros(4, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dx, dl = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(logits, torch.ones_like(logits))
+        for call in (lambda: node_attention(dx, x, x, p), lambda: node_attention(x, dx, x, p),
+                     lambda: node_attention(x, x, dx, p),
+                     lambda: node_attention(x, x, x, p, dist=torch.zeros(6, 6),
+                                            slope=forward_ad.make_dual(torch.ones(2), torch.ones(2))),
+                     lambda: dropout_add(dx, rng, 0.5), lambda: dropout_add(x, rng, 0.5, residual=dx),
+                     lambda: action_log_probs(dl, act)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        # without one the call goes on, here to where there is no device
+        with pytest.raises(ValueError, match="HIP device"):
+            node_attention(x, x, x, p)
