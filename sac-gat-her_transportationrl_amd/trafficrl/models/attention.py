@@ -111,8 +111,8 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
     A row that sees no node gives zeros and passes no gradient.  Entries of q,
     k, v and the gradient must be finite, or a network's own rows (no other
     network's) may become NaN.  max_queries / max_nodes: the largest network's
-    rows; hints that shape the launch.  Give them where a batch holds many
-    small networks: without, it takes several times as long.
+    rows; hints that shape the launch, taken from dist's shape where it is given.
+    Without either, a batch of many small networks takes several times as long.
 
     Differentiable once in q, k, v and slope (a forward-mode tangent is refused).
     Scores, softmax statistics and sums are float32; with half types the
@@ -161,8 +161,10 @@ def node_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ptr: torch
         raise ValueError(f"{what}: scale must be finite, cap finite and >= 0 (got {scale}, {cap})")
     if cap > 0.0 and not abs(scale) < cap * 1e30:
         raise ValueError(f"{what}: cap {cap} is too small beside scale {scale}")
-    max_queries = rows if max_queries is None else int(max_queries)
-    max_nodes = nodes if max_nodes is None else int(max_nodes)
+    # the distances' shape bounds the largest network; a single one is bounded by its rows
+    most_q, most_k = dist.shape[-2:] if dist is not None and ptr.numel() > 2 else (rows, nodes)
+    max_queries = min(rows, most_q) if max_queries is None else int(max_queries)
+    max_nodes = min(nodes, most_k) if max_nodes is None else int(max_nodes)
     if max_queries < 0 or max_nodes < 0:
         raise ValueError(f"{what}: max_queries and max_nodes must be >= 0")
     no_tangents(what, q, k, v, dist, slope)

@@ -145,3 +145,40 @@ def test_tangents_are_refused():
         # without one the call goes on, here to where there is no device
         with pytest.raises(ValueError, match="HIP device"):
             node_attention(x, x, x, p)
+
+
+def test_distances_bound_the_launch(no_library, monkeypatch):
+    """Without hints a launch is shaped by dist, which holds the largest of several networks; a single one by its rows."""
+    from trafficrl import _lib
+    from trafficrl.models import node_attention
+    seen = []
+
+    class Keep(_Recorder):
+        def trx_node_attention_forward(self, a, stream):
+            seen.append((a.max_queries, a.max_nodes))
+            return 0
+    monkeypatch.setattr(_lib, "load", lambda: Keep())
+    x, many, one = torch.zeros(48, 2, 32), torch.tensor([0, 24, 48]), torch.tensor([0, 48])
+    q, qp = torch.zeros(2, 2, 32), torch.tensor([0, 1, 2])
+    for kw, want in [
+            (dict(dist=torch.zeros(24, 24)), (24, 24)), (dict(dist=torch.zeros(2, 30, 26)), (30, 26)),
+            (dict(dist=torch.zeros(90, 90)), (48, 48)), (dict(), (48, 48)),
+            (dict(dist=torch.zeros(24, 24), max_queries=7, max_nodes=9), (7, 9)),
+            (dict(ptr=one, dist=torch.zeros(5, 5)), (48, 48)),
+            (dict(q=q, ptr=qp, k_ptr=many, dist=torch.zeros(1, 24)), (1, 24))]:
+        a = dict(q=x, ptr=many) | kw
+        node_attention(a.pop("q"), x, x, a.pop("ptr"), **a)
+        assert seen[-1] == want, kw
+
+
+@pytest.mark.gpu
+def test_launch_shaped_by_distances():
+    """The same bits as with the hints given; a matrix smaller than the networks leaves no row out."""
+    from trafficrl.models import node_attention
+    from test_node_attention import assert_within, ints, make, reference
+    q, k, v, p, _, dist, slope, _ = make([24] * 40 + [7, 90], 4, 2, 32, torch.bfloat16, "shared", seed=6)
+    a = node_attention(q, k, v, ints(p), dist=dist, slope=slope)
+    assert torch.equal(a, node_attention(q, k, v, ints(p), dist=dist, slope=slope, max_queries=90, max_nodes=90))
+    small = dist[:10, :5].contiguous()
+    out = node_attention(q, k, v, ints(p), dist=small, slope=slope)
+    assert_within("out", out, *reference(q, k, v, p, p, small, slope)["out"])
