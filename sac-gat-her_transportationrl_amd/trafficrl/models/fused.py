@@ -31,7 +31,7 @@ import torch.nn.functional as F
 
 from .. import _lib
 from .gat_encoder import GATEncoder, GraphCSR, _LoopMean, build_csr, is_regular_batch
-from .tensor_cache import TensorKeyed, pin
+from .tensor_cache import TensorKeyed, owner
 
 
 @dataclass
@@ -702,18 +702,16 @@ def tail_infer(model, x_prev: torch.Tensor, ea: torch.Tensor, a_all: torch.Tenso
     return logits, out
 
 
-_idx32_cache: Dict[Tuple, torch.Tensor] = {}
+_idx32_cache = TensorKeyed()
 
 
 def _idx32(t: torch.Tensor) -> torch.Tensor:
-    key = (t.data_ptr(), t._version, t.numel(), t.device)
+    key = (t.data_ptr(), t._version, t.shape, t.stride(), t.device)
     r = _idx32_cache.get(key)
     if r is None:
         r = t.to(torch.int32).contiguous()
-        if len(_idx32_cache) > 64:
-            _idx32_cache.clear()
-        _idx32_cache[key] = r
-    return pin(r)
+        _idx32_cache.put(key, (owner(t),), r)
+    return r
 
 
 def _edge_args(p, c, ea, we, w2, b2, src32, dst32, B: int, n: int, E: int):

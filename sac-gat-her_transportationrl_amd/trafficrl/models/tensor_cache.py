@@ -34,6 +34,13 @@ def pinning():
         _PIN_STACK.pop()
 
 
+def owner(t):
+    """The tensor that lives as long as t's memory does: what t is a view of, or t
+    itself.  A view such as edge_index[0] is a new object in every call, so an
+    entry that lived as long as it would never be found again."""
+    return t._base if t._is_view() else t
+
+
 class TensorKeyed:
     """Cache keyed by tensors' (address, version, ...).  An entry is valid only
     while the tensors it was computed from are alive: a new tensor allocated

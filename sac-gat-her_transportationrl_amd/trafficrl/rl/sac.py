@@ -30,6 +30,7 @@ import torch.nn.functional as F
 from ..models import fused
 from ..models.gat_encoder import GATEncoder, is_regular_batch
 from ..models.skinny import regular_gather, skinny_linear, splitk_linear
+from ..models.tensor_cache import TensorKeyed, owner
 from .policy import ActionLogProbs, action_log_probs
 
 
@@ -112,7 +113,7 @@ def segment_softmax(logits: torch.Tensor, index: torch.Tensor, num: int, per_seg
     return ex / (scatter_sum(ex, index, num)[index] + 1e-16)
 
 
-_edge_layout_cache: dict = {}
+_edge_layout_cache = TensorKeyed()
 
 
 def is_regular_edges(edge_index: torch.Tensor, batch: torch.Tensor, num_graphs: int) -> bool:
@@ -127,13 +128,11 @@ def is_regular_edges(edge_index: torch.Tensor, batch: torch.Tensor, num_graphs: 
     if r is None:
         eb = batch[edge_index[0]].long()
         r = bool(torch.equal(eb, torch.arange(num_graphs, device=eb.device).repeat_interleave(E // num_graphs)))
-        if len(_edge_layout_cache) > 64:
-            _edge_layout_cache.clear()
-        _edge_layout_cache[key] = r
+        _edge_layout_cache.put(key, (owner(edge_index), owner(batch)), r)
     return r
 
 
-_regular_cache: Dict[Tuple, Tuple] = {}
+_regular_cache = TensorKeyed()
 
 
 def regular_layout(edge_index: torch.Tensor, batch: torch.Tensor, num_graphs: int):
@@ -153,9 +152,7 @@ def regular_layout(edge_index: torch.Tensor, batch: torch.Tensor, num_graphs: in
             loc = edge_index.long() - (torch.arange(B, device=edge_index.device) * n).repeat_interleave(m)
             loc = loc.view(2, B, m)
             r = (B, loc[0, 0].contiguous(), loc[1, 0].contiguous()) if bool((loc == loc[:, :1]).all()) else False
-        if len(_regular_cache) > 64:
-            _regular_cache.clear()
-        _regular_cache[key] = r
+        _regular_cache.put(key, (owner(edge_index), owner(batch)), r)
     return r if r is not False else None
 
 
