@@ -409,9 +409,11 @@ constexpr float kFarBack = sizeof(T) == 2 ? 1024.0f : kFar;
 // two-byte types, a tile whose arguments all lie within a quarter of zero takes the series to x^7 (off by 4e-7 of x at
 // the end), seven operations; others 1 - 2 / (1 + e^2x) by the hardware's exp2 and reciprocal, twelve, off by 2^-23:
 // 8e-6 in a score at a cap of 64, far below what rounding its probability takes.  With larger caps that error would
-// grow past the scores' own, so there arguments within a quarter of zero take the series wherever they are.
+// grow past the scores' own, so there arguments within a quarter of zero take the series wherever they are.  So they do
+// where `alone`: a score is then the same number in whatever tile it is computed.  The backward passes need that beside
+// biases so large that the least difference moves the sum to its neighbour, which may weigh 2^90 times as much.
 template <typename T, int kTiles, bool SLACK>
-__device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles], float pre, float cap) {
+__device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles], float pre, float cap, bool alone) {
     if constexpr (sizeof(T) == 4) {
         TRX_EACH_SCORE {
             const float th = tanhf(s[n][r] * pre);
@@ -434,7 +436,7 @@ __device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kT
                 s[n][r] = cap * th;
                 if (SLACK) slack[n][r] = __builtin_fmaf(-th, th, 1.0f);
             }
-        } else if (cap <= 64.0f) {
+        } else if (cap <= 64.0f && !alone) {
             TRX_EACH_SCORE {
                 const float e = exp2_fast(s[n][r] * (2.0f * kLog2e));
                 const float th = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
@@ -453,9 +455,9 @@ __device__ __forceinline__ void cap_scores(f32x4 (&s)[kTiles], f32x4 (&slack)[kT
 }
 // the products of a tile to scores: with the scale, or capped
 template <typename T, bool CAP, bool SLACK, int kTiles>
-__device__ __forceinline__ void scores(const Call& call, f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles]) {
+__device__ __forceinline__ void scores(const Call& call, f32x4 (&s)[kTiles], f32x4 (&slack)[kTiles], bool alone) {
     if (CAP) {
-        cap_scores<T, kTiles, SLACK>(s, slack, call.unit.pre, call.a.cap);
+        cap_scores<T, kTiles, SLACK>(s, slack, call.unit.pre, call.a.cap, alone);
     } else if (call.unit.pre != 1.0f) {
         TRX_EACH_SCORE s[n][r] *= call.unit.pre;
     }

@@ -183,7 +183,7 @@ attention_bwd_q_kernel(Call call, RowSums out, float* part) {
                         d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + d_row[t] + 16 * n + 4 * g);
                 }
                 f32x4 slack[kTiles];
-                scores<T, CAP, true>(call, s[t], slack);
+                scores<T, CAP, true>(call, s[t], slack, far[t]);
                 if (DIST) {
                     // beside weights of zero a distance must not be infinite in the slopes' sums
                     if (__all(slope[t] < 0.0f) && ordinary(d[t])) {
@@ -469,7 +469,7 @@ attention_bwd_kv_kernel(Call call, const float* dots, const float* inverse, floa
 #pragma unroll
             for (int t = 0; t < MK; ++t) {
                 f32x4 slack[kTiles];
-                scores<T, CAP, true>(call, s[t], slack);
+                scores<T, CAP, true>(call, s[t], slack, far);
                 if (DIST) {
                     if (falls && ordinary(d[t])) {
                         TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope[n][r], d[t][n][r], s[t][n][r]);

@@ -137,7 +137,7 @@ attention_fwd_kernel(Call call, float* part) {
                     for (int n = 0; n < kTiles; ++n)
                         d[t][n] = *reinterpret_cast<const f32x4*>(d_tile + d_row[t] + 16 * n + 4 * g);
                 }
-                scores<T, CAP, false>(call, s[t], s[t]);
+                scores<T, CAP, false>(call, s[t], s[t], false);
                 if (DIST) {
                     if (__all(slope[t] < 0.0f) && ordinary(d[t])) {   // a distance of +inf makes its -inf by itself
                         TRX_EACH_SCORE s[t][n][r] = __builtin_fmaf(slope[t], d[t][n][r], s[t][n][r]);

@@ -112,3 +112,25 @@ def test_weights_sum_to_one(shape, dt, cap):
             near = (2 * HALF[dt] + (nk + 2 * nq + 64) * U + 2.0 ** -14 * (dt != F32)) * rows.abs().sum((0, 2))
             near = near + (HALF[dt] + U) * got["v"][kp[b]:kp[b + 1]].double().abs().sum(0) + nk * 2.0 ** -25
             assert bool(((have - rows.sum((0, 2))).abs() <= near).all()), (far, b)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("n", [24, 40, 200])
+def test_capped_scores_do_not_depend_on_their_tile(dt, n):
+    """Scores of 1e-9 beside a bias that lies halfway between two float32 numbers 64 apart: their sum's rounding hangs
+    on the last bit of the capped score.  One large score among them sends some tiles another way; both backward
+    passes must still see the same scores, or a row's weights do not sum to one."""
+    m = 7000001                                    # 1 mod 4: the tie goes to the number below
+    q, k = (torch.zeros(n, 1, 16, device="cuda", dtype=dt) for _ in range(2))
+    q[..., 0], k[..., 0] = 2.0 ** -14, 2.0 ** -14
+    q[..., 1] = 1.0
+    k[min(20, n - 1), 0, 1] = 8.0
+    g = torch.Generator("cuda").manual_seed(n)
+    v, go = (torch.randn(n, 1, 16, device="cuda", generator=g).to(dt) for _ in range(2))
+    dist = torch.full((n, n), 128.0 * m, device="cuda")
+    got = run(q, k, v, go, dist, torch.full((1,), 0.75, device="cuda"), [0, n], [0, n], scale=0.25, cap=3.0)
+    have, rows = got["v"].double().sum(0), go.double()
+    near = (2 * HALF[dt] + (3 * n + 64) * U + 2.0 ** -14 * (dt != F32)) * rows.abs().sum(0)
+    near = near + (HALF[dt] + U) * got["v"].double().abs().sum(0) + n * 2.0 ** -25
+    assert bool(((have - rows.sum(0)).abs() <= near).all())
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
