@@ -879,10 +879,11 @@ int trx_episode_step(int32_t num_envs, const double* reward, const uint8_t* done
  * channels]: contiguous, in dtype.  lse float32 [num_queries, heads]:
  * log(sum_j e^w), written by the forward where not NULL (-inf for an empty
  * row), read by the backward, which sums the weights around it anew: what its
- * rounding loses where a row's scores are large and alike does not count.  out_low: like out, or NULL: what rounding
- * took from out; with it the backward's <grad_out, out> is as exact as in
- * float32.  grad_slope float32 [heads] or NULL (NULL without slope or dist).
- * max_queries / max_nodes: the largest graph's rows; they only shape the
+ * rounding loses where a row's scores are large and alike does not count.
+ * out_low: like out, or NULL: what rounding took from out, in dtype too; with
+ * both the backward's <grad_out, out> has out to 2^-17 in bfloat16, in float16
+ * to 2^-23 or 2^-25 absolute.  grad_slope float32 [heads] or NULL (NULL without
+ * slope or dist).  max_queries / max_nodes: the largest graph's rows; they only shape the
  * launch (a smaller value costs time, never rows).  Sums and the softmax's
  * statistics are float32; probabilities and score gradients enter the matrix
  * products in dtype.  Deterministic: no float atomics.  At most 2^23 / heads

@@ -14,7 +14,8 @@ namespace {
 // all and a workgroup of four would idle.  The axis that is run over is split where the tiles that there are about
 // leave compute units without work, into pieces of at least `least` rows (a piece costs its accumulator's round trip),
 // up to 64 and 256 MB.  512 workgroups of four waves, two to a compute unit: 4001 nodes, 8 heads of 64, forward and
-// backward together 396 us, against 587 us with 256 and 434 us with 1024.
+// backward together 396 us, against 587 us with 256 and 434 us with 1024 (compared side by side; the passes have
+// changed by a few percent since).
 AttentionCut cut(int64_t kept, int64_t run, int64_t all, int64_t graphs, int64_t heads, int64_t row_bytes, int wide,
                  int least) {
     AttentionCut c;

@@ -15,11 +15,16 @@
 // 0.0042 where the softmax is peaked; with out_low 0.0024 to 0.0025.  Inputs of
 // mean zero gain nothing.  out_low costs 0.5 us forward and 2 us here at 4001 nodes.
 //
-// What bounds them: as forward, vector instructions (12.7 and 13.8 a score, issuing
-// in 45% and 38% of the cycles, the matrix pipe busy in 20%) and waiting, with two
-// waves a SIMD.  4001 nodes, 8 heads of 64, bfloat16, distances: 134 us (grad_q) and
-// 150 us (grad_k, grad_v), 288 TFLOP/s of the five products that are needed; 4096
-// nodes without distances 189 us together with the sums (455 TFLOP/s).
+// p and u are rounded to the type for their products, as the forward's weights are
+// (float16's range is kept, see Raise).  Gradients in bfloat16 are off by 0.0024
+// (relative to float64) where rounding the results alone costs 0.0017.
+//
+// What bounds them: as forward, vector instructions (15.0 and 15.4 a score, issuing
+// in 50% and 40% of the cycles, the matrix pipe busy in 19%) and waiting (36% and 52%
+// of the waves' cycles), with two waves a SIMD.  4001 nodes, 8 heads of 64, bfloat16,
+// distances: 132 us (grad_q) and 154 us (grad_k, grad_v), 280 TFLOP/s of the five
+// products that are needed with the sums; 4096 nodes without distances 192 us
+// together with the sums (448 TFLOP/s).
 #pragma once
 #include <algorithm>
 

@@ -7,14 +7,20 @@
 // of the group), so a shared head's keys are read once.  Keys, values and
 // distances pass through LDS in tiles of KT, the next tile on its way in registers.
 //
+// Weights are rounded to the type for the product with v, because the matrix
+// instructions take operands of it; their sum is not.  Results in bfloat16 are off
+// by 0.0019 to 0.0020 (relative to float64), where rounding the result alone costs
+// 0.0016 to 0.0017.
+//
 // What bounds it.  Large graphs: the vector instructions of the scores and waiting.
-// 4096 nodes, 8 heads of 64, bfloat16, with distances: 10.7 vector instructions a
-// score issue in 47% of the cycles, the matrix pipe is busy in 16%; registers
-// allow two waves a SIMD (three: 183 us against 132 when tried).  Times at 4096
-// nodes, 8 heads, bfloat16: 110 us at 128 channels (628 TFLOP/s), 76 at 64 (452);
-// with distances 142 and 107.  64 keys a tile at 64 channels with distances (32:
-// 120 us against 107), 32 at 128.  Small graphs and single queries: memory.  4096
-// networks of 24 nodes, 4 heads of 64: 42 us (201 MB at 4.8 TB/s, a large copy's
+// 4096 nodes, 8 heads of 64, bfloat16, with distances: 11.8 vector instructions a
+// score issue in 50% of the cycles, the matrix pipe is busy in 16%, waves wait in
+// 31% of theirs; registers allow two waves a SIMD (three: 183 us against 132 when
+// tried).  With the splits' join, 4096 nodes, 8 heads, bfloat16: 110 us at 128
+// channels (623 TFLOP/s), 72 to 78 at 64 (442 to 477); with distances 145 and 100.
+// 64 keys a tile at 64 channels with distances (32: 120 us against 107 when tried),
+// 32 at 128.  Small graphs and single queries: memory.  4096
+// networks of 24 nodes, 4 heads of 64: 43 us (201 MB at 4.7 TB/s, a large copy's
 // rate); 8 queries over 32768 nodes each, 16 heads on 2 of 128: 50 us and 7 us for
 // joining the splits (270 MB at 4.7 TB/s together).
 #pragma once
