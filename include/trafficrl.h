@@ -933,8 +933,8 @@ int trx_node_attention_backward(const trx_node_attention_args* a, void* stream);
  * Backward: grad_logits (dtype; rows contiguous, row_len apart, or packed like
  * the logits) = g_log_prob (1[j = action] - p_j) - g_entropy p_j (log p_j +
  * entropy) + sum_t g_top[t] (1[j = top_action[t]] - p_j); 0 where a link may
- * not be chosen, and for packed elements of no row; an action of log_prob -inf
- * passes nothing.  The g_* may be NULL.  max_row: the longest packed row; it
+ * not be chosen, and for packed elements of no row; an action that may not be
+ * chosen, or outside its row, passes nothing.  The g_* may be NULL.  max_row: the longest packed row; it
  * only shapes the launch.  At most 2^23 rows, 2^30 links in one.  workspace: trx_action_log_probs_workspace_bytes
  * bytes, 16-byte aligned (0: may be NULL; the forward's only).             */
 #define TRX_TOP_MAX 16
