@@ -400,7 +400,7 @@ struct Raise {
 };
 constexpr float kRaiseAll = 0x1p100f;   // until something has been seen
 // In the backward passes R comes from lse, and near zero two-byte types take the weights around it for probabilities:
-// they sum to 1 within 2^-14 up to 2^10, below a 2^5th of such a type's own step.
+// up to 2^10 their sum is 1 within 2^-14 (half a step of lse and one of c), an eighth of half a step of float16.
 template <typename T>
 constexpr float kFarBack = sizeof(T) == 2 ? 1024.0f : kFar;
 // what is done to every score of a lane's column: n over its tiles, r over a tile's four rows
